@@ -148,6 +148,81 @@ class EmaSpanStateArgs(ctypes.Structure):
     ]
 
 
+class DeltaFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("seqlen", _i64), ("nheads", _i64), ("headdim", _i64), ("dstate", _i64), ("ngroups", _i64),
+        ("nseq", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+        ("q", _ptr), ("q_stride", _i64 * 3),
+        ("k", _ptr), ("k_stride", _i64 * 3),
+        ("v", _ptr), ("v_stride", _i64 * 3),
+        ("g", _ptr), ("beta", _ptr), ("cu_seqlens", _ptr), ("initial_states", _ptr),
+        ("out", _ptr), ("out_stride", _i64 * 3),
+        ("final_states", _ptr),
+        ("workspace", _ptr), ("workspace_bytes", ctypes.c_size_t),
+        ("saved", _ptr), ("saved_bytes", ctypes.c_size_t),
+    ]
+
+
+class DeltaBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("seqlen", _i64), ("nheads", _i64), ("headdim", _i64), ("dstate", _i64), ("ngroups", _i64),
+        ("nseq", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+        ("q", _ptr), ("q_stride", _i64 * 3),
+        ("k", _ptr), ("k_stride", _i64 * 3),
+        ("v", _ptr), ("v_stride", _i64 * 3),
+        ("g", _ptr), ("beta", _ptr), ("cu_seqlens", _ptr),
+        ("saved", _ptr), ("saved_bytes", ctypes.c_size_t),
+        ("dout", _ptr), ("dout_stride", _i64 * 3),
+        ("d_final_states", _ptr),
+        ("dq", _ptr), ("dq_stride", _i64 * 3),
+        ("dk", _ptr), ("dk_stride", _i64 * 3),
+        ("dv", _ptr), ("dv_stride", _i64 * 3),
+        ("dg", _ptr), ("dbeta", _ptr), ("d_initial_states", _ptr),
+        ("workspace", _ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class DeltaStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("tokens", _i64), ("nheads", _i64), ("headdim", _i64), ("dstate", _i64), ("ngroups", _i64),
+        ("slots", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+        ("q", _ptr), ("q_stride", _i64 * 3),
+        ("k", _ptr), ("k_stride", _i64 * 3),
+        ("v", _ptr), ("v_stride", _i64 * 3),
+        ("g", _ptr), ("beta", _ptr),
+        ("states", _ptr), ("state_stride", _i64 * 2),
+        ("state_indices", _ptr),
+        ("out", _ptr), ("out_stride", _i64 * 3),
+    ]
+
+
+class GatedNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("group_size", _i64),
+        ("dtype", _i32), ("weight_dtype", _i32), ("norm_before_gate", _i32), ("eps", ctypes.c_float),
+        ("x", _ptr), ("x_stride", _i64), ("z", _ptr), ("z_stride", _i64), ("weight", _ptr),
+        ("y", _ptr), ("y_stride", _i64),
+        ("dy", _ptr), ("dy_stride", _i64), ("dx", _ptr), ("dx_stride", _i64), ("dz", _ptr), ("dz_stride", _i64),
+        ("dweight", _ptr), ("workspace", _ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64),
+        ("dtype", _i32), ("residual_dtype", _i32), ("weight_dtype", _i32), ("eps", ctypes.c_float),
+        ("scale", ctypes.c_float), ("reserved", _i32),
+        ("x", _ptr), ("x_stride", _i64), ("residual", _ptr), ("residual_stride", _i64), ("weight", _ptr),
+        ("y", _ptr), ("y_stride", _i64), ("h", _ptr), ("h_stride", _i64),
+        ("dy", _ptr), ("dy_stride", _i64), ("dh", _ptr), ("dh_stride", _i64), ("dx", _ptr), ("dx_stride", _i64),
+        ("d_residual", _ptr), ("d_residual_stride", _i64),
+        ("dweight", _ptr), ("workspace", _ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 lib.ema_scan_workspace_size.restype = ctypes.c_size_t
 lib.ema_scan_workspace_size.argtypes = [_i64] * 5
 lib.ema_fwd_launch.restype = ctypes.c_int
@@ -199,6 +274,18 @@ lib.ema_p2p_close.restype = ctypes.c_int
 lib.ema_p2p_close.argtypes = [_ptr]
 lib.ssd_device_status.restype = ctypes.c_int
 lib.ssd_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), ctypes.c_int, _ptr]
+for _name, _args in (("delta_fwd_launch", DeltaFwdArgs), ("delta_bwd_launch", DeltaBwdArgs),
+                     ("delta_step_launch", DeltaStepArgs), ("gated_norm_fwd_launch", GatedNormArgs),
+                     ("gated_norm_bwd_launch", GatedNormArgs), ("residual_norm_fwd_launch", ResidualNormArgs),
+                     ("residual_norm_bwd_launch", ResidualNormArgs)):
+    getattr(lib, _name).restype = ctypes.c_int
+    getattr(lib, _name).argtypes = [ctypes.POINTER(_args), _ptr]
+lib.delta_workspace_bytes.restype = ctypes.c_size_t
+lib.delta_workspace_bytes.argtypes = [_i64] * 7 + [_i32] * 2
+lib.delta_saved_bytes.restype = ctypes.c_size_t
+lib.delta_saved_bytes.argtypes = [_i64] * 7 + [_i32]
+lib.block_norm_workspace_bytes.restype = ctypes.c_size_t
+lib.block_norm_workspace_bytes.argtypes = [_i64] * 3
 lib.ema_last_error.restype = ctypes.c_char_p
 lib.ema_version.restype = ctypes.c_char_p
 

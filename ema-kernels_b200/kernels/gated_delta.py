@@ -1,0 +1,319 @@
+"""The gated delta rule on the B200 kernels: whole sequences (autograd) and the recurrent step.
+
+Per sequence and head, a state S (headdim x dstate, fp32) with the decay a_t = exp(g_t):
+
+    S_t = a_t S_{t-1} + beta_t (v_t - a_t S_{t-1} k_t) k_t^T,    o_t = scale S_t q_t
+
+Layouts are those of the SSD scan (kernels.ssd_combined): v and o (batch, seqlen, nheads, headdim), q and k
+(batch, seqlen, ngroups, dstate) shared by the nheads / ngroups heads of a group, g and beta (batch,
+seqlen, nheads), states (sequences, nheads, headdim, dstate).  The keys are taken as given: a model that
+wants unit keys normalises them first.  The reference has no delta rule; no reference file stands behind this.
+
+* :func:`gated_delta_rule` -- training and prefill, chunks of 64 tokens, forward and backward, plain
+  batches or sequences packed end to end (``cu_seqlens``).
+* :func:`gated_delta_step` -- decoding: one or a few tokens per row on a cache of states, updated in place.
+
+bf16 / fp16 / fp32 q, k, v; dstate 64 or 128; headdim a multiple of 8 up to 128 (256 for the step).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+__all__ = ["gated_delta_rule", "gated_delta_step"]
+
+_DSTATES = (64, 128)
+
+
+def _check(q, k, v, g, beta, what):
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and g.is_cuda and beta.is_cuda):
+        raise ValueError(f"{what}: q, k, v, g and beta must be on CUDA")
+    if not (q.device == k.device == v.device == g.device == beta.device):
+        raise ValueError(f"{what}: q, k, v, g and beta must be on one device")
+    if v.ndim != 4 or q.ndim != 4:
+        raise ValueError(f"{what}: q, k (batch, seqlen, ngroups, dstate), v (batch, seqlen, nheads, headdim)")
+    b, length, H, V = v.shape
+    G, K = q.shape[2], q.shape[3]
+    if q.shape != (b, length, G, K) or k.shape != q.shape:
+        raise ValueError(f"{what}: q and k must be (batch, seqlen, ngroups, dstate), got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)} for v {tuple(v.shape)}")
+    if g.shape != (b, length, H) or beta.shape != (b, length, H):
+        raise ValueError(f"{what}: g and beta must be (batch, seqlen, nheads)")
+    if G == 0 or H == 0 or H % G:
+        raise ValueError(f"{what}: nheads {H} must be a multiple of ngroups {G}")
+    if v.dtype not in _lib.DTYPE_CODES or q.dtype != v.dtype or k.dtype != v.dtype:
+        raise ValueError(f"{what}: q, k and v must share one of bf16, fp16, fp32")
+    if K not in _DSTATES:
+        raise ValueError(f"{what}: dstate must be 64 or 128, got {K}")
+    return b, length, H, V, G, K
+
+
+def _check_headdim(V, most, what):
+    if V == 0 or V % 8 or V > most:
+        raise ValueError(f"{what}: headdim must be a multiple of 8 up to {most}, got {V}")
+
+
+def _rows(t):
+    """t itself where its rows can be addressed as they are: unit last stride, 16-byte steps and base."""
+    es = t.element_size()
+    steps = [s for s, n in zip(t.stride()[:3], t.shape) if n > 1]
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any((s * es) % 16 for s in steps):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t):
+    """Element strides of the three outer axes; an axis of one element, whatever its stride, takes a row's step."""
+    return (_lib._i64 * 3)(*(s if n > 1 else t.shape[3] for s, n in zip(t.stride()[:3], t.shape)))
+
+
+def _f32(t):
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
+def _set_shape(a, dims, nseq, dtype, scale):
+    a.batch, a.seqlen, a.nheads, a.headdim, a.ngroups, a.dstate = dims
+    a.nseq, a.dtype, a.scale = nseq, _lib.DTYPE_CODES[dtype], scale
+
+
+def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, want_final, save):
+    """One forward launch: (o, final states or None, what a backward needs or None)."""
+    b, length, H, V = v.shape
+    G, K = q.shape[2], q.shape[3]
+    dims = (b, length, H, V, G, K)
+    nseq = b if cu_seqlens is None else cu_seqlens.numel() - 1
+    dev = v.device
+    q, k, v, g, beta = _rows(q), _rows(k), _rows(v), _f32(g), _f32(beta)
+    # a packed call's tokens outside every sequence get zeros
+    o = (torch.empty if cu_seqlens is None else torch.zeros)(b, length, H, V, dtype=v.dtype, device=dev)
+    final = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_final else None
+    a = _lib.DeltaFwdArgs()
+    _set_shape(a, dims, nseq, v.dtype, scale)
+    size = (b, length, nseq, H, V, K, G, a.dtype)
+    nbytes = _lib.lib.delta_saved_bytes(*size) if save else _lib.lib.delta_workspace_bytes(*size, 0)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    a.q, a.q_stride, a.k, a.k_stride = q.data_ptr(), _strides(q), k.data_ptr(), _strides(k)
+    a.v, a.v_stride, a.out, a.out_stride = v.data_ptr(), _strides(v), o.data_ptr(), _strides(o)
+    a.g, a.beta, a.cu_seqlens = g.data_ptr(), beta.data_ptr(), _lib.ptr(cu_seqlens)
+    s0 = None if initial_states is None else _f32(initial_states)
+    a.initial_states, a.final_states = _lib.ptr(s0), _lib.ptr(final)
+    if save:
+        a.saved, a.saved_bytes = buf.data_ptr(), nbytes
+    else:
+        a.workspace, a.workspace_bytes = buf.data_ptr(), nbytes
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib.delta_fwd_launch(a, _lib.stream_ptr(dev)), "gated_delta_rule")
+    return o, final, buf if save else None
+
+
+def _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial):
+    """One backward launch: (dq, dk, dv, dg, dbeta, d initial states or None); dg, dbeta fp32."""
+    b, length, H, V = v.shape
+    G, K = q.shape[2], q.shape[3]
+    nseq = b if cu_seqlens is None else cu_seqlens.numel() - 1
+    dev = v.device
+    q, k, v, g, beta, do = _rows(q), _rows(k), _rows(v), _f32(g), _f32(beta), _rows(do.to(v.dtype))
+    new = torch.empty if cu_seqlens is None else torch.zeros
+    dq, dk = (new(b, length, G, K, dtype=v.dtype, device=dev) for _ in range(2))
+    dv = new(b, length, H, V, dtype=v.dtype, device=dev)
+    dg, dbeta = (new(b, length, H, dtype=torch.float32, device=dev) for _ in range(2))
+    ds0 = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_d_initial else None
+    a = _lib.DeltaBwdArgs()
+    _set_shape(a, (b, length, H, V, G, K), nseq, v.dtype, scale)
+    nbytes = _lib.lib.delta_workspace_bytes(b, length, nseq, H, V, K, G, a.dtype, 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    for name, t in (("q", q), ("k", k), ("v", v), ("dout", do), ("dq", dq), ("dk", dk), ("dv", dv)):
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride", _strides(t))
+    a.g, a.beta, a.cu_seqlens, a.dg, a.dbeta = (g.data_ptr(), beta.data_ptr(), _lib.ptr(cu_seqlens), dg.data_ptr(),
+                                                dbeta.data_ptr())
+    a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
+    ds1 = None if d_final is None else _f32(d_final)
+    a.d_final_states, a.d_initial_states = _lib.ptr(ds1), _lib.ptr(ds0)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib.delta_bwd_launch(a, _lib.stream_ptr(dev)), "gated_delta_rule backward")
+    return dq, dk, dv, dg, dbeta, ds0
+
+
+# ---- dispatcher operators: torch.compile traces them, autograd through register_autograd ----
+def _empty0(like):
+    return like.new_empty((0,), dtype=torch.float32)
+
+
+@torch.library.custom_op("ema_b200::delta_fwd", mutates_args=(), device_types="cuda")
+def _delta_fwd_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                  initial_states: Optional[torch.Tensor], cu_seqlens: Optional[torch.Tensor],
+                  scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(o, the final states, what the backward reads)."""
+    return _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, True, True)
+
+
+@_delta_fwd_op.register_fake
+def _(q, k, v, g, beta, initial_states, cu_seqlens, scale):
+    b, length, H, V = v.shape
+    G, K = q.shape[2], q.shape[3]
+    nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    nbytes = _lib.lib.delta_saved_bytes(b, length, nseq, H, V, K, G, _lib.DTYPE_CODES[v.dtype])
+    return (v.new_empty((b, length, H, V)), v.new_empty((nseq, H, V, K), dtype=torch.float32),
+            v.new_empty((nbytes,), dtype=torch.uint8))
+
+
+@torch.library.custom_op("ema_b200::delta_bwd", mutates_args=(), device_types="cuda")
+def _delta_bwd_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                  cu_seqlens: Optional[torch.Tensor], saved: torch.Tensor, do: torch.Tensor,
+                  d_final: Optional[torch.Tensor], scale: float,
+                  want_d_initial: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                                 torch.Tensor]:
+    """(dq, dk, dv, dg, dbeta, d initial states), the last empty when not wanted."""
+    *grads, ds0 = _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial)
+    return (*grads, ds0 if ds0 is not None else _empty0(v))
+
+
+@_delta_bwd_op.register_fake
+def _(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial):
+    b, length, H, V = v.shape
+    G, K = q.shape[2], q.shape[3]
+    nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    f32 = torch.float32
+    return (q.new_empty((b, length, G, K)), q.new_empty((b, length, G, K)), v.new_empty((b, length, H, V)),
+            v.new_empty((b, length, H), dtype=f32), v.new_empty((b, length, H), dtype=f32),
+            v.new_empty((nseq, H, V, K), dtype=f32) if want_d_initial else _empty0(v))
+
+
+def _setup(ctx, inputs, output):
+    q, k, v, g, beta, initial_states, cu_seqlens, scale = inputs
+    ctx.save_for_backward(q, k, v, g, beta, cu_seqlens, output[2])
+    ctx.scale = scale
+    ctx.d_initial = initial_states is not None and ctx.needs_input_grad[5]
+    ctx.initial_dtype = None if initial_states is None else initial_states.dtype
+    ctx.set_materialize_grads(False)
+
+
+def _backward(ctx, do, d_final, _d_saved):
+    q, k, v, g, beta, cu, saved = ctx.saved_tensors
+    if do is None and d_final is None:
+        return (None,) * 8
+    if do is None:
+        do = torch.zeros_like(v)
+    dq, dk, dv, dg, dbeta, ds0 = torch.ops.ema_b200.delta_bwd(q, k, v, g, beta, cu, saved, do, d_final, ctx.scale,
+                                                              ctx.d_initial)
+    return (dq, dk, dv, dg.to(g.dtype), dbeta.to(beta.dtype), ds0.to(ctx.initial_dtype) if ctx.d_initial else None,
+            None, None)
+
+
+torch.library.register_autograd("ema_b200::delta_fwd", _backward, setup_context=_setup)
+
+
+def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_final_states=False, cu_seqlens=None):
+    """o (batch, seqlen, nheads, headdim), or (o, final states) with ``return_final_states``.
+
+    g is the log decay (not positive in a decaying layer; at or below -100 the state is dropped), beta the write
+    strength, ``scale`` defaults to dstate ** -0.5.  ``initial_states`` (sequences, nheads, headdim, dstate)
+    is the state before the first token.  ``cu_seqlens`` (nseq + 1, int32 or int64, on the device) packs
+    sequences into a batch of one: sequence n is tokens [cu[n], cu[n + 1]), of any length, zero too
+    (its final state is its initial one); tokens outside every sequence give zeros.
+
+    Gradients: q, k, v, g, beta and initial_states; those of a group's q and k sum over its heads.  The states,
+    all sums and both gate gradients are fp32."""
+    b, length, H, V, G, K = _check(q, k, v, g, beta, "gated_delta_rule")
+    _check_headdim(V, 128, "gated_delta_rule")
+    nseq = b
+    if cu_seqlens is not None:
+        if b != 1:
+            raise ValueError("gated_delta_rule: packed sequences come as a batch of one")
+        if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("gated_delta_rule: cu_seqlens must be (nseq + 1,) int32 or int64")
+        if cu_seqlens.device != v.device:
+            raise ValueError("gated_delta_rule: cu_seqlens must be on v's device")
+        nseq = cu_seqlens.numel() - 1
+        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+    if initial_states is not None:
+        if initial_states.shape != (nseq, H, V, K) or initial_states.device != v.device:
+            raise ValueError(f"gated_delta_rule: initial_states must be {(nseq, H, V, K)} on v's device, got "
+                             f"{tuple(initial_states.shape)}")
+    scale = K ** -0.5 if scale is None else float(scale)
+    wants = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states))
+    if wants or torch.compiler.is_compiling():
+        o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale)
+    else:
+        o, final, _ = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, return_final_states, False)
+    return (o, final) if return_final_states else o
+
+
+def _delta_step(q, k, v, g, beta, states, state_indices, scale):
+    b, T, H, V = v.shape
+    o = torch.empty(b, T, H, V, dtype=v.dtype, device=v.device)
+    q, k, g, beta = _rows(q), _rows(k), _f32(g), _f32(beta)
+    if v.stride(3) != 1:
+        v = v.clone(memory_format=torch.contiguous_format)
+    a = _lib.DeltaStepArgs()
+    a.batch, a.tokens, a.nheads, a.headdim, a.dstate, a.ngroups = b, T, H, V, q.shape[3], q.shape[2]
+    a.slots, a.dtype, a.scale = states.shape[0], _lib.DTYPE_CODES[v.dtype], scale
+    a.q, a.q_stride, a.k, a.k_stride = q.data_ptr(), _strides(q), k.data_ptr(), _strides(k)
+    a.v, a.v_stride, a.out, a.out_stride = v.data_ptr(), _strides(v), o.data_ptr(), _strides(o)
+    a.g, a.beta, a.states, a.state_indices = (g.data_ptr(), beta.data_ptr(), states.data_ptr(),
+                                              _lib.ptr(state_indices))
+    a.state_stride = (_lib._i64 * 2)(states.stride(0), states.stride(1))
+    with torch.cuda.device(v.device):
+        _lib.check(_lib.lib.delta_step_launch(a, _lib.stream_ptr(v.device)), "gated_delta_step")
+    return o
+
+
+@torch.library.custom_op("ema_b200::delta_step", mutates_args=("states",), device_types="cuda")
+def _delta_step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                   states: torch.Tensor, state_indices: Optional[torch.Tensor], scale: float) -> torch.Tensor:
+    return _delta_step(q, k, v, g, beta, states, state_indices, scale)
+
+
+@_delta_step_op.register_fake
+def _(q, k, v, g, beta, states, state_indices, scale):
+    return torch.empty_like(v, memory_format=torch.contiguous_format)
+
+
+def gated_delta_step(q, k, v, g, beta, states, scale=None, state_indices=None):
+    """The recurrent form for decoding: o (batch, tokens, nheads, headdim), ``states`` updated in place.
+
+    q, k (batch, tokens, ngroups, dstate), v (batch, tokens, nheads, headdim), g, beta (batch, tokens,
+    nheads), tokens usually one; the token axis may be left out of all of them (and is then left out of o).  ``states``
+    (slots, nheads, headdim, dstate) fp32 is the cache; row b works on slot ``state_indices[b]`` (int32 or
+    int64 on the device; b itself when None).  An index outside the cache marks an idle row: its output is zero and no
+    state changes.  Rows of one call must not share a slot.  No gradient."""
+    squeeze = v.ndim == 3
+    if squeeze:
+        q, k, v, g, beta = (t.unsqueeze(1) for t in (q, k, v, g, beta))
+    b, _, H, V, _, K = _check(q, k, v, g, beta, "gated_delta_step")
+    _check_headdim(V, 256, "gated_delta_step")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, states)):
+        raise ValueError("gated_delta_step has no gradient: call it under torch.no_grad() or use gated_delta_rule")
+    if states.ndim != 4 or states.shape[1:] != (H, V, K) or states.dtype != torch.float32:
+        raise ValueError(f"gated_delta_step: states must be (slots, {H}, {V}, {K}) fp32, got {tuple(states.shape)} "
+                         f"{states.dtype}")
+    if states.device != v.device:
+        raise ValueError("gated_delta_step: states must be on v's device")
+    if states.stride(3) != 1 or states.stride(2) != K or states.data_ptr() % 16 or any(
+            s % 4 for s in states.stride()[:2]):
+        raise ValueError("gated_delta_step: the (headdim, dstate) block of a state must be contiguous, 16-byte aligned")
+    if state_indices is None:
+        if states.shape[0] < b:
+            raise ValueError(f"gated_delta_step: {b} rows on {states.shape[0]} slots")
+    else:
+        if state_indices.shape != (b,) or state_indices.dtype not in (torch.int32, torch.int64):
+            raise ValueError("gated_delta_step: state_indices must be (batch,) int32 or int64")
+        if state_indices.device != v.device:
+            raise ValueError("gated_delta_step: state_indices must be on v's device")
+        if state_indices.dtype == torch.int64:
+            # clamped before the narrowing, so that a huge index stays outside the cache
+            state_indices = state_indices.clamp(-1, states.shape[0])
+        state_indices = state_indices.to(torch.int32).contiguous()
+    scale = K ** -0.5 if scale is None else float(scale)
+    if torch.compiler.is_compiling():
+        o = torch.ops.ema_b200.delta_step(q, k, v, g, beta, states, state_indices, scale)
+    else:
+        o = _delta_step(q, k, v, g, beta, states, state_indices, scale)
+    return o.squeeze(1) if squeeze else o
