@@ -1,0 +1,650 @@
+// Gated delta rule, tensor-core family: the gradients of q, k, g and beta, chunk by chunk and in parallel, once the
+// forward walk has left S0 and E and the backward walk dS1 and dX (formulas in delta_common.cuh).
+//
+// With lanes as token rows (M = 128: 64 query rows over 64 key rows, [dO; dX] and [Q; K]) one chain gives both
+// 64 x 64 matrices of a head and one the products they are weighted with:
+//   [dO; dX] E^t = [f; F'],   [Q; K] K^t = [qk; kk]
+//   N = scale Gam f beta, M = -Gam F' beta (bf16, for dq and dk);  y = scale Gam f qk  over  -Gam F' kk
+// with lanes as state columns (M = dstate) everything that ends in dq or dk:
+//   a1 = S0^t dO^t, a2 = S0^t dX^t, a3 = dS1^t E^t, a4 = K^t N^t, a5 = K^t (M + M^t) + Q^t N
+//   dq = scale exp(b) a1 + a4,   dk = -exp(b) a2 + beta w a3 + a5      (w_j = exp(b_end - b_j))
+// and what the gates need, by transposed butterflies over the lanes of fp32 values:
+//   dbeta_j = sum of y over its column + w_j k_j . a3_j
+//   dg_t = sum over rows of (prefix of beta y up to t) + sum_{i >= t} r_i + sum_{j < t} c_j + exp(b_end) <dS1, S0>
+// dg and dbeta are fp32 results, so S0, dS1, E and dX enter as hi + lo pairs wherever they reach them (delta_tc.cuh).
+// N is a pair too where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are single bf16.
+//
+// One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  Bound: the
+// images' bytes (S0 and dS1 are 2 x 64 KB a chunk and head at 128 x 128) and, near it, the epilogues.  Roles: warps
+// 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 <dS1, S0> and the gates' results, warp 12 the MMAs,
+// warp 13 the loads.  S0 hi and dS1 hi stay for the whole head, one more slot takes S0 lo and then dS1 lo.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "delta_host.h"
+#include "delta_tc.cuh"
+#include "ema_scan_dispatch.h"
+
+namespace emab {
+namespace delta {
+namespace {
+
+constexpr int kEpi = 8, kAux = 4;
+constexpr int kMma = 12, kLoad = 13;  // (14 and 15 only fill their warpgroup)
+constexpr int kThreads = 16 * 32;
+constexpr int kRegEpi = 184, kRegAux = 72, kRegCtl = 72;
+static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128, "register split");
+constexpr int kReg = 128 * 128;  // two 64-row tiles of 64 columns, one over the other
+
+// tensor-memory columns
+constexpr uint32_t cKQ = 0;     // [qk; kk]
+constexpr uint32_t cF = 64;     // [f; F'] of E hi, of E lo, then of dX lo (its rows alone); a4 and a5 after them
+constexpr uint32_t cA = 256;    // a1, a2
+constexpr uint32_t cA3 = 384;   // a3 of E hi, of E lo
+
+struct Bars {
+  uint64_t qk_full, qk_empty, ox_full, ox_empty, ex_full, ex_empty;
+  uint64_t a_full, a_empty, b_full, b_empty, c_full, c_empty;  // S0 hi, dS1 hi, the lo slot
+  uint64_t g_full[2], g_empty[2];
+  uint64_t f, a, a3, a45;      // MMA groups done
+  uint64_t nm, free;           // N, M written; all accumulators read
+  uint64_t sums, fin;          // the epilogues' sums written; dg, dbeta done with them
+  uint64_t epi_sync, aux_sync; // meetings of the epilogue warps, of warps 8-11 (bounded, unlike a barrier instruction)
+  uint64_t drain;
+  uint32_t taddr, fail;
+};
+
+struct Small {
+  float gate[2][kGateFloats];
+  float y[4][kC], r[4][kC], R[4][kC], c[4][kC];  // column sums by lane quarter
+  float base[128];                                // row sums of a row's first 32 columns
+  float dot[kAux];
+  Bars bar;
+};
+
+// Offsets from the 1024-byte aligned base, by the padded channel count.
+template <int K>
+struct Layout {
+  int ox, ex, sa, sb, sc, nm, out, small;
+  __host__ __device__ explicit Layout(int VP) {
+    const int img = VP * 128, st = VP * K * 2;
+    ox = (K / 64) * kReg;                       // after [Q; K]
+    ex = ox + (VP / 64) * kReg;                 // E hi, E lo, dX lo
+    sa = ex + 3 * img;
+    sb = sa + st;
+    sc = sb + st;
+    const int end = sc + st;
+    nm = VP == 128 ? ex + 2 * img : end;        // N, M: over dX lo once a1, a2 and F' have read it
+    out = VP == 128 ? end : end + 2 * kTile;    // N lo; 32 rows of dq or dk on their way out
+    small = out + kTile;                        // (32 x dstate bf16 fit it)
+  }
+  __host__ __device__ int bytes() const { return small + static_cast<int>(sizeof(Small)); }
+};
+
+// Column sums over the warp's 32 lanes: lane l gets column l.
+__device__ __forceinline__ float column_sums(float (&x)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float give = up ? x[i] : x[i + o];
+      x[i] = (up ? x[i + o] : x[i]) + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  return x[0];
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float (&v)[32]) {
+  float a[16], b[16];
+  tc::tmem_ld16(at, a);
+  tc::tmem_ld16(at + 16, b);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    v[i] = a[i];
+    v[16 + i] = b[i];
+  }
+}
+
+template <int K>
+__global__ void __launch_bounds__(kThreads, 1)
+    grads_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq,
+                    const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap mdv, const Params p,
+                    const TcBuffers w, uint32_t* status) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int VP = pad_channels(p.V), img = VP * 128, simg = VP * K * 2;
+  const Layout<K> lay(VP);
+  Small& sm = *reinterpret_cast<Small*>(smem + lay.small);
+  Bars& bar = sm.bar;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hpg = p.H / p.G;
+  const int tasks = p.slots * p.G;
+  volatile uint32_t* fail = &bar.fail;
+
+  if (tid == 0) {
+    uint64_t* one[] = {&bar.qk_full, &bar.ox_full, &bar.ox_empty, &bar.ex_full, &bar.ex_empty, &bar.a_full, &bar.b_full,
+                       &bar.c_full, &bar.g_full[0], &bar.g_full[1], &bar.f, &bar.a, &bar.a3, &bar.a45, &bar.fin,
+                       &bar.drain};
+    for (uint64_t* b : one) mbar_init(b, 1);
+    mbar_init(&bar.qk_empty, 1 + kEpi);
+    mbar_init(&bar.a_empty, 1 + kAux);
+    mbar_init(&bar.b_empty, 1 + kAux);
+    mbar_init(&bar.c_empty, 1 + kAux);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.g_empty[i], kEpi + 1);
+    mbar_init(&bar.nm, kEpi);
+    mbar_init(&bar.free, kEpi);
+    mbar_init(&bar.sums, kEpi);
+    mbar_init(&bar.epi_sync, kEpi);
+    mbar_init(&bar.aux_sync, kAux);
+    bar.fail = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMma) tc::tmem_alloc(&bar.taddr, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  constexpr uint32_t tb = 0;  // the whole of tensor memory is this block's: its base is 0 (checked below)
+  if (bar.taddr != 0u) {
+    if (tid == 0) {
+      atomicOr(status, kStatusTmem);
+      bar.fail = 1;
+    }
+    __syncthreads();
+  }
+  auto wait1 = [&](uint64_t* b, uint32_t parity) { return chain_wait(b, parity, status, fail); };
+  auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait1(b, parity)) != 0; };
+  uint32_t meetings = 0;
+  auto meet = [&](uint64_t* b) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(b);
+    return wait(b, meetings++ & 1);
+  };
+
+  if (warp >= kMma) {
+    set_regs_down<kRegCtl>();
+    if (warp == kLoad && lane == 0) {  // ---- loads
+      int n, tok, task = 0, hc = 0;    // tasks and heads begun
+      Seq q;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
+        const int slot = t / p.G, gr = t - slot * p.G;
+        if (!chunk_at(p, slot, &n, &q, &tok)) continue;
+        const int tt = q.t0 + tok;
+        if (task > 0 && !(ok = wait1(&bar.qk_empty, (task - 1) & 1))) break;
+        mbar_arrive_expect_tx(&bar.qk_full, (K / 64) * kReg);
+        for (int i = 0; i < K / 64; ++i) {
+          tma_load_4d(smem + i * kReg, &mq, &bar.qk_full, 64 * i, gr, tt, q.b);
+          tma_load_4d(smem + i * kReg + kTile, &mk, &bar.qk_full, 64 * i, gr, tt, q.b);
+        }
+        ++task;
+        for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
+          const long long ch = static_cast<long long>(slot) * p.H + h;
+          const uint32_t last = (hc - 1) & 1;
+          if (hc > 1 && !(ok = wait1(&bar.g_empty[hc & 1], (hc / 2 - 1) & 1))) break;
+          mbar_arrive_expect_tx(&bar.g_full[hc & 1], kGateFloats * 4);
+          bulk_g2s(sm.gate[hc & 1], w.gates + ch * kGateFloats, kGateFloats * 4, &bar.g_full[hc & 1]);
+          if (hc > 0 && !(ok = wait1(&bar.ox_empty, last))) break;
+          mbar_arrive_expect_tx(&bar.ox_full, (VP / 64) * kReg);
+          for (int i = 0; i < VP / 64; ++i) {
+            tma_load_4d(smem + lay.ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
+            tma_load_4d(smem + lay.ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
+          }
+          if (hc > 0 && !(ok = wait1(&bar.ex_empty, last))) break;
+          mbar_arrive_expect_tx(&bar.ex_full, 3 * img);
+          bulk_g2s(smem + lay.ex, w.E + ch * 2 * img, 2 * img, &bar.ex_full);
+          bulk_g2s(smem + lay.ex + 2 * img, w.dX + ch * img, img, &bar.ex_full);
+          if (hc > 0 && !(ok = wait1(&bar.a_empty, last))) break;
+          mbar_arrive_expect_tx(&bar.a_full, simg);
+          bulk_g2s(smem + lay.sa, w.S + ch * 2 * simg, simg, &bar.a_full);
+          if (hc > 0 && !(ok = wait1(&bar.c_empty, 1))) break;  // two phases a head: the last one's second
+          mbar_arrive_expect_tx(&bar.c_full, simg);
+          bulk_g2s(smem + lay.sc, w.S + ch * 2 * simg + simg, simg, &bar.c_full);
+          if (hc > 0 && !(ok = wait1(&bar.b_empty, last))) break;
+          mbar_arrive_expect_tx(&bar.b_full, simg);
+          bulk_g2s(smem + lay.sb, w.dS + ch * 2 * simg, simg, &bar.b_full);
+          if (!(ok = wait1(&bar.c_empty, 0))) break;
+          mbar_arrive_expect_tx(&bar.c_full, simg);
+          bulk_g2s(smem + lay.sc, w.dS + ch * 2 * simg + simg, simg, &bar.c_full);
+        }
+      }
+      if (!ok) {  // failed: what was begun lands before the block ends (each barrier's last phase, or an earlier one)
+        const long long t0 = clock64();
+        while (clock64() - t0 < kWaitLimitCycles / 100) __nanosleep(1000);
+      }
+    }
+    if (warp == kMma) {  // ---- MMAs
+      constexpr uint32_t idKQ = tc::idesc_bf16(128, 64, false, false);
+      constexpr uint32_t idF = tc::idesc_bf16(128, 128, false, true);
+      constexpr uint32_t idA = tc::idesc_bf16(128, 128, true, false);
+      constexpr uint32_t idMM128 = tc::idesc_bf16(128, 128, true, true);
+      constexpr uint32_t idMM = tc::idesc_bf16(128, 64, true, true);
+      constexpr uint32_t idMK = tc::idesc_bf16(128, 64, true, false);
+      auto kstep = [](int s) { return static_cast<uint64_t>(((s >> 2) * kReg + (s & 3) * 32) >> 4); };
+      auto nstep = [](int s) { return static_cast<uint64_t>((s * 2048) >> 4); };
+      auto jstep = [](int s) { return static_cast<uint64_t>((s * 32) >> 4); };
+      const uint32_t sb = smem_u32(smem);
+      // state columns as lanes: two 64-column regions (dstate 64: the same one twice, the upper lanes are not read)
+      const uint32_t sreg = K == 128 ? static_cast<uint32_t>(img) : 0u, qreg = K == 128 ? kReg : 0u;
+      const uint64_t dQK = tc::smem_desc_sw128(sb, 16, 1024), dK = tc::smem_desc_sw128(sb + kTile, 16, 1024);
+      const uint64_t dQn = tc::smem_desc_sw128(sb, qreg, 1024), dKn = tc::smem_desc_sw128(sb + kTile, qreg, 1024);
+      const uint64_t dOX = tc::smem_desc_sw128(sb + lay.ox, 16, 1024);
+      const uint64_t dE = tc::smem_desc_sw128(sb + lay.ex, img, 1024);         // [E hi | E lo]
+      const uint64_t dEX = tc::smem_desc_sw128(sb + lay.ex, 2 * img, 1024);    // [E hi | dX lo]
+      const uint64_t dXl = tc::smem_desc_sw128(sb + lay.ex + 2 * img, img, 1024);
+      const uint64_t dSA = tc::smem_desc_sw128(sb + lay.sa, sreg, 1024), dSB = tc::smem_desc_sw128(sb + lay.sb, sreg, 1024);
+      const uint64_t dSC = tc::smem_desc_sw128(sb + lay.sc, sreg, 1024);
+      const uint64_t dN = tc::smem_desc_sw128(sb + lay.nm, 16, 1024), dM = tc::smem_desc_sw128(sb + lay.nm + kTile, 16, 1024);
+      const uint64_t dNl = tc::smem_desc_sw128(sb + lay.out, 16, 1024);
+      const int vs = VP / 16;
+      int n, tok, task = 0, hc = 0;
+      Seq q;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
+        const int slot = t / p.G, gr = t - slot * p.G;
+        if (!chunk_at(p, slot, &n, &q, &tok)) continue;
+        const int have = q.len - tok;
+        const bool cut = have < kC && p.cu != nullptr;  // rows of the next sequence in the tiles
+        ok = wait(&bar.qk_full, task & 1);
+        if (!ok) break;
+        if (cut) {
+          zero_rows(smem, K / 64, kReg, have);
+          zero_rows(smem + kTile, K / 64, kReg, have);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        ++task;
+        for (int h = 0; h < hpg; ++h, ++hc) {
+          const uint32_t ph = hc & 1;
+          ok = wait(&bar.ox_full, ph) && wait(&bar.ex_full, ph);
+          if (!ok) break;
+          if (cut) {
+            zero_rows(smem + lay.ox, VP / 64, kReg, have);
+            zero_rows(smem + lay.ox + kTile, VP / 64, kReg, have);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (hc > 0) ok = wait(&bar.free, (hc - 1) & 1);
+          if (!ok) break;
+          tc::fence_after_sync();
+          if (elect_one()) {
+            if (h == 0) {
+#pragma unroll
+              for (int s = 0; s < K / 16; ++s) tc::mma_bf16(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
+            }
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cF, dOX + kstep(s), dE + nstep(s), idF, s > 0);
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cF + 128, dEX + nstep(s), dE + nstep(s), idMM, s > 0);
+            tc::mma_commit(&bar.f);
+          }
+          __syncwarp();
+          ok = wait(&bar.a_full, ph);
+          if (!ok) break;
+          if (elect_one()) {
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA, dSA + nstep(s), dOX + kstep(s), idA, s > 0);
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA + 64, dSA + nstep(s), dXl + nstep(s), idMM, true);
+            tc::mma_commit(&bar.a_empty);
+          }
+          __syncwarp();
+          ok = wait(&bar.c_full, 0);
+          if (!ok) break;
+          if (elect_one()) {
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA, dSC + nstep(s), dOX + kstep(s), idA, true);
+            tc::mma_commit(&bar.a);
+            tc::mma_commit(&bar.c_empty);
+            tc::mma_commit(&bar.ox_empty);
+          }
+          __syncwarp();
+          ok = wait(&bar.b_full, ph);
+          if (!ok) break;
+          if (elect_one()) {
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA3, dSB + nstep(s), dE + nstep(s), idMM128, s > 0);
+            tc::mma_commit(&bar.b_empty);
+          }
+          __syncwarp();
+          ok = wait(&bar.c_full, 1);
+          if (!ok) break;
+          if (elect_one()) {
+            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA3, dSC + nstep(s), dE + nstep(s), idMM, true);
+            tc::mma_commit(&bar.a3);
+            tc::mma_commit(&bar.c_empty);
+          }
+          __syncwarp();
+          ok = wait(&bar.nm, ph);
+          if (!ok) break;
+          tc::fence_after_sync();
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + nstep(s), idMM, true);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
+            tc::mma_commit(&bar.a45);
+            tc::mma_commit(&bar.ex_empty);
+            if (h == hpg - 1) tc::mma_commit(&bar.qk_empty);
+          }
+          __syncwarp();
+        }
+      }
+      if (*fail != 0u && elect_one()) {
+        tc::mma_commit(&bar.drain);
+        mbar_wait_bounded(&bar.drain, 0, status);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= kEpi) {  // ---- <dS1, S0>, dg, dbeta
+    set_regs_down<kRegAux>();
+    const int at = tid - kEpi * 32;
+    int n, tok, hc = 0;
+    Seq q;
+    bool ok = true;
+    auto dot8 = [](uint4 a, uint4 b, float2 acc) {
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc = f2_fma(cvt_pair<__nv_bfloat16>(x[i]), cvt_pair<__nv_bfloat16>(y[i]), acc);
+      return acc;
+    };
+    auto dot = [&](int x, int y, float2 acc) {  // of two state images (the same element in the same place)
+#pragma unroll 4
+      for (int i = at * 16; i < simg; i += kAux * 32 * 16)
+        acc = dot8(*reinterpret_cast<const uint4*>(smem + x + i), *reinterpret_cast<const uint4*>(smem + y + i), acc);
+      return acc;
+    };
+    auto release = [&](uint64_t* b) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b);
+    };
+    for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
+      const int slot = t / p.G, gr = t - slot * p.G;
+      if (!chunk_at(p, slot, &n, &q, &tok)) continue;
+      for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
+        const uint32_t ph = hc & 1;
+        ok = wait(&bar.a_full, ph) && wait(&bar.c_full, 0) && wait(&bar.b_full, ph);
+        if (!ok) break;
+        float2 acc = dot(lay.sa, lay.sb, make_float2(0, 0));
+        float2 low = dot(lay.sc, lay.sb, make_float2(0, 0));  // S0 lo dS1 hi
+        release(&bar.c_empty);
+        release(&bar.b_empty);
+        ok = wait(&bar.c_full, 1);
+        if (!ok) break;
+        low = dot(lay.sa, lay.sc, low);
+        release(&bar.c_empty);
+        release(&bar.a_empty);
+        float d = (acc.x + acc.y) + (low.x + low.y);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (lane == 0) sm.dot[warp - kEpi] = d;
+        ok = meet(&bar.aux_sync);
+        if (ok && warp == kEpi) {
+          ok = wait(&bar.g_full[hc & 1], (hc / 2) & 1) && wait(&bar.sums, ph);
+          if (ok) {
+            const float* gate = sm.gate[hc & 1];
+            const float all = ((sm.dot[0] + sm.dot[1]) + (sm.dot[2] + sm.dot[3])) * gate[kGateEnd];
+            float y[2], r[2], R[2], c[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int j = 2 * lane + k;
+              y[k] = (sm.y[0][j] + sm.y[1][j]) + (sm.y[2][j] + sm.y[3][j]);
+              r[k] = (sm.r[0][j] + sm.r[1][j]) + (sm.r[2][j] + sm.r[3][j]);
+              R[k] = (sm.R[0][j] + sm.R[1][j]) + (sm.R[2][j] + sm.R[3][j]);
+              c[k] = (sm.c[0][j] + sm.c[1][j]) + (sm.c[2][j] + sm.c[3][j]);  // w_j k_j . a3_j
+            }
+            const float b0 = gate[kGateBeta + 2 * lane], b1 = gate[kGateBeta + 2 * lane + 1];
+            float pre = b0 * c[0] + b1 * c[1], suf = r[0] + r[1];  // sums up to and from this lane's tokens
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float a = __shfl_up_sync(0xffffffffu, pre, o), b = __shfl_down_sync(0xffffffffu, suf, o);
+              if (lane >= o) pre += a;
+              if (lane + o < 32) suf += b;
+            }
+            const float before = __shfl_up_sync(0xffffffffu, pre, 1);
+            const float after = __shfl_down_sync(0xffffffffu, suf, 1);
+            const float pre0 = lane > 0 ? before : 0.f, suf1 = r[1] + (lane < 31 ? after : 0.f);
+            const float dg[2] = {R[0] + (suf1 + r[0]) + pre0 + all, R[1] + suf1 + (pre0 + b0 * c[0]) + all};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int j = 2 * lane + k;
+              if (tok + j < q.len) {
+                const long long to = (static_cast<long long>(q.b) * p.L + q.t0 + tok + j) * p.H + h;
+                p.dg[to] = p.g[to] > kMinGate ? dg[k] : 0.f;  // a clamped gate has no gradient
+                p.dbeta[to] = y[k] + c[k];
+              }
+            }
+          }
+          __syncwarp();
+          if (ok && lane == 0) {
+            mbar_arrive(&bar.fin);
+            mbar_arrive(&bar.g_empty[hc & 1]);
+          }
+          __syncwarp();
+        }
+        ok = ok && meet(&bar.aux_sync);  // sm.dot has been read
+        if (!ok) break;
+      }
+    }
+  } else {  // ---- epilogues
+    set_regs_up<kRegEpi>();
+    const int quarter = warp & 3, hf = warp >> 2, row = 32 * quarter + lane, c0 = 32 * hf;
+    const uint32_t tl = static_cast<uint32_t>(32 * quarter) << 16;
+    const bool klive = row < K;
+    int n, tok, hc = 0;
+    Seq q;
+    bool ok = true;
+    auto arrive = [&](uint64_t* b) {
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b);
+    };
+    for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
+      const int slot = t / p.G, gr = t - slot * p.G;
+      if (!chunk_at(p, slot, &n, &q, &tok)) continue;
+      float dq[32], dk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dq[i] = dk[i] = 0.f;
+      for (int h = 0; h < hpg; ++h, ++hc) {
+        const uint32_t ph = hc & 1;
+        const float* gate = sm.gate[hc & 1];
+        ok = wait(&bar.g_full[hc & 1], (hc / 2) & 1) && wait(&bar.f, ph);
+        if (!ok) break;
+        tc::fence_after_sync();
+        {  // rows: f and qk (lanes 0-63), F' and kk (64-127); columns c0 ..
+          const int i = row & 63;
+          const bool second = quarter >= 2;
+          float x[32];
+          {
+            float a[32];
+            tmem_ld32(tb + tl + cF + c0, x);
+            tmem_ld32(tb + tl + cF + 64 + c0, a);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] += a[k];
+            if (second) {
+              tmem_ld32(tb + tl + cF + 128 + c0, a);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] += a[k];
+            }
+          }
+          const float bi = gate[kGateB + i];
+          const float sc = second ? -1.f : p.scale;
+          const int lim = second ? i - 1 : i;  // last column of the row
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[k] = c0 + k <= lim ? sc * __expf(bi - gate[kGateB + c0 + k]) * x[k] : 0.f;
+          ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
+          ok = ok && wait(&bar.a, ph);                   // dX lo has been read where N and M go
+          if (!ok) break;
+          unsigned char* tile = smem + lay.nm + (second ? kTile : 0);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t o[4], l[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const float2 be = *reinterpret_cast<const float2*>(gate + kGateBeta + c0 + 8 * k + 2 * m);
+              split2(f2_mul(be, make_float2(x[8 * k + 2 * m], x[8 * k + 2 * m + 1])), o[m], l[m]);
+            }
+            const uint32_t to = tc::chunk_off(i, 4 * hf + k);
+            *reinterpret_cast<uint4*>(tile + to) = make_uint4(o[0], o[1], o[2], o[3]);
+            if (!second) *reinterpret_cast<uint4*>(smem + lay.out + to) = make_uint4(l[0], l[1], l[2], l[3]);
+          }
+          fence_proxy_async_smem();
+          float prod[32];
+          tmem_ld32(tb + tl + cKQ + c0, prod);
+          tc::tmem_wait_ld();
+          arrive(&bar.nm);
+          // y, and the prefixes of beta y along the row that reach column t <= i
+          float R[32], run = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            x[k] *= prod[k];
+            R[k] = run;
+            run = fmaf(gate[kGateBeta + c0 + k], x[k], run);
+          }
+          if (hf == 0) sm.base[row] = run;
+          const float y = column_sums(x, lane);
+          ok = meet(&bar.epi_sync);
+          if (!ok) break;
+          const float base = hf == 0 ? 0.f : sm.base[row];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) R[k] = c0 + k <= i ? R[k] + base : 0.f;
+          const float Rs = column_sums(R, lane);
+          sm.y[quarter][c0 + lane] = y;
+          sm.R[quarter][c0 + lane] = Rs;
+        }
+        // state columns as lanes: a1, a2, a3 (bar.a has completed)
+        tc::fence_after_sync();
+        {
+          const unsigned char* tq = smem + (K == 128 ? (row >> 6) * kReg : 0);
+          const uint32_t col = (row & 63) * 2;
+          auto elem = [&](const unsigned char* tile, int tk) {
+            return klive ? to_f32(*reinterpret_cast<const __nv_bfloat16*>(tile + tk * 128 + (col ^ ((tk & 7) << 4)))) : 0.f;
+          };
+          float s[32];
+          {
+            float a[32];
+            tmem_ld32(tb + tl + cA + c0, a);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float v = -p.scale * gate[kGateE + c0 + k] * a[k];
+              dq[k] += v;
+              s[k] = v * elem(tq, c0 + k);
+            }
+            tmem_ld32(tb + tl + cA + 64 + c0, a);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float v = gate[kGateE + c0 + k] * a[k];
+              dk[k] += v;
+              s[k] = klive ? fmaf(v, elem(tq + kTile, c0 + k), s[k]) : 0.f;
+            }
+          }
+          sm.r[quarter][c0 + lane] = column_sums(s, lane);
+          ok = wait(&bar.a3, ph);
+          if (!ok) break;
+          tc::fence_after_sync();
+          {
+            float a[32], b[32];
+            tmem_ld32(tb + tl + cA3 + c0, a);
+            tmem_ld32(tb + tl + cA3 + 64 + c0, b);
+            tc::tmem_wait_ld();
+            const float end = gate[kGateB + kC - 1];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float v = a[k] + b[k];
+              dk[k] = fmaf(gate[kGateW + c0 + k], v, dk[k]);
+              s[k] = klive ? __expf(end - gate[kGateB + c0 + k]) * v * elem(tq + kTile, c0 + k) : 0.f;
+            }
+          }
+          sm.c[quarter][c0 + lane] = column_sums(s, lane);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.sums);
+          mbar_arrive(&bar.g_empty[hc & 1]);
+        }
+        ok = wait(&bar.a45, ph);
+        if (!ok) break;
+        tc::fence_after_sync();
+        {
+          float a[32], b[32];
+          tmem_ld32(tb + tl + cF + c0, a);
+          tmem_ld32(tb + tl + cF + 64 + c0, b);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            dq[k] += a[k];
+            dk[k] += b[k];
+          }
+        }
+        arrive(&bar.free);
+      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&bar.qk_empty);  // (its tiles were last read before bar.sums)
+      // dq and dk, 32 tokens at a time: through a tile in shared memory to whole 16-byte pieces of their rows
+      const int have = min(kC, q.len - tok);
+#pragma unroll
+      for (int part = 0; part < 4; ++part) {
+        const int which = part >> 1, half = part & 1;
+        ok = meet(&bar.epi_sync);  // the tile's last pieces have been read
+        if (!ok) break;
+        if (klive && hf == half) {
+          uint16_t* so = reinterpret_cast<uint16_t*>(smem + lay.out) + row;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const uint32_t v = which == 0 ? pack_pair<__nv_bfloat16>(make_float2(dq[k], dq[k + 1]))
+                                          : pack_pair<__nv_bfloat16>(make_float2(dk[k], dk[k + 1]));
+            so[k * K] = static_cast<uint16_t>(v);
+            so[(k + 1) * K] = static_cast<uint16_t>(v >> 16);
+          }
+        }
+        ok = meet(&bar.epi_sync);
+        if (!ok) break;
+        constexpr int kPieces = K / 8, kRows = kEpi * 32 / kPieces;
+        const int pc = tid % kPieces;
+        void* out = which == 0 ? p.dq : p.dk;
+        const View& v = which == 0 ? p.vdq : p.vdk;
+        for (int tk = tid / kPieces; tk < 32 && 32 * half + tk < have; tk += kRows)
+          __stcs(reinterpret_cast<uint4*>(row_of<__nv_bfloat16>(out, v, q.b, q.t0 + tok + 32 * half + tk, gr)) + pc,
+                 *reinterpret_cast<const uint4*>(smem + lay.out + (tk * kPieces + pc) * 16));
+      }
+      ok = ok && meet(&bar.epi_sync);  // N lo of the next head goes where they were
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == kMma) {
+    tc::tmem_relinquish();
+    tc::tmem_dealloc(bar.taddr, 512);
+  }
+}
+
+template <int K>
+cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mq, const CUtensorMap& mo, const CUtensorMap& mdv,
+                   const Params& p, const TcBuffers& w, uint32_t* status, cudaStream_t st) {
+  static unsigned long long mask = 0;
+  const int most = Layout<K>(128).bytes() > Layout<K>(64).bytes() ? Layout<K>(128).bytes() : Layout<K>(64).bytes();
+  cudaError_t e = static_cast<cudaError_t>(
+      ensure_smem_attr(reinterpret_cast<const void*>(grads_tc_kernel<K>), most, &mask));
+  if (e != cudaSuccess) return e;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const long long tasks = static_cast<long long>(p.slots) * p.G;
+  grads_tc_kernel<K><<<static_cast<unsigned>(tasks < sms ? tasks : sms), kThreads, Layout<K>(pad_channels(p.V)).bytes(),
+                       st>>>(mk, mq, mo, mdv, p, w, status);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t tc_grads(const CUtensorMap& mk, const CUtensorMap& mq, const CUtensorMap& mo, const CUtensorMap& mdv,
+                     const Params& p, const TcBuffers& w, uint32_t* status, cudaStream_t st) {
+  if (p.slots == 0) return cudaSuccess;
+  return p.K == 64 ? launch<64>(mk, mq, mo, mdv, p, w, status, st) : launch<128>(mk, mq, mo, mdv, p, w, status, st);
+}
+
+}  // namespace delta
+}  // namespace emab

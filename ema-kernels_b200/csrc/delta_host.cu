@@ -7,12 +7,15 @@
 #include <cstdio>
 
 #include "delta_b200.h"
+#include "ema_scan_dispatch.h"
 
 namespace emab {
 void set_last_error(const char* msg);
 
 namespace delta {
 namespace {
+
+__device__ uint32_t g_status;  // error word of the tensor-core kernels
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -40,12 +43,47 @@ int64_t slots_bound(int64_t batch, int64_t seqlen, int64_t nseq) {
 struct Carver {
   char* base;
   size_t at = 0;
-  float* take(size_t n) {
-    float* p = base != nullptr ? reinterpret_cast<float*>(base + at) : nullptr;
-    at += (n * 4 + 255) / 256 * 256;
+  char* bytes(size_t n) {
+    char* p = base != nullptr ? base + at : nullptr;
+    at += (n + 255) / 256 * 256;
     return p;
   }
+  float* take(size_t n) { return reinterpret_cast<float*>(bytes(n * 4)); }
 };
+
+size_t carve_tc_fwd(TcBuffers* w, char* base, int64_t slots, int64_t H, int64_t V, int64_t K, bool keep) {
+  Carver c{base};
+  const size_t n = static_cast<size_t>(slots) * H;
+  w->gates = c.take(n * kGateFloats);
+  w->T = c.bytes(n * 2 * kTile);
+  w->P = c.bytes(n * 2 * kTile);
+  w->S = keep ? c.bytes(n * 2 * state_image(static_cast<int>(V), static_cast<int>(K))) : nullptr;
+  w->E = keep ? c.bytes(n * 2 * token_image(static_cast<int>(V))) : nullptr;
+  return c.at;
+}
+size_t carve_tc_bwd(TcBuffers* w, char* base, int64_t slots, int64_t H, int64_t V, int64_t K) {
+  Carver c{base};
+  const size_t n = static_cast<size_t>(slots) * H;
+  w->dS = c.bytes(n * 2 * state_image(static_cast<int>(V), static_cast<int>(K)));
+  w->dX = c.bytes(n * token_image(static_cast<int>(V)));
+  return c.at;
+}
+// The tensor-core kernels take bf16 (every dstate and headdim of the entry points); a call without tokens, whose
+// tiles no tensor map can describe, goes to the fp32 family, which then only copies the states.
+bool on_tensor_cores(int dtype, int64_t seqlen, int flags) {
+  return dtype == EMA_DTYPE_BF16 && seqlen > 0 && (flags & DELTA_FP32_PRODUCTS) == 0;
+}
+
+// Tiles of 64 tokens of one head of a (batch, token, head, channel) tensor: `box` channels, swizzled or as they are.
+int tile_map(CUtensorMap* m, const void* t, const int64_t (&st)[3], int64_t channels, int64_t heads, int64_t seqlen,
+             int64_t batch, int64_t box, bool swizzle) {
+  const uint64_t d[4] = {static_cast<uint64_t>(channels), static_cast<uint64_t>(heads), static_cast<uint64_t>(seqlen),
+                         static_cast<uint64_t>(batch)};
+  const uint64_t s[3] = {static_cast<uint64_t>(st[2]) * 2, static_cast<uint64_t>(st[1]) * 2,
+                         static_cast<uint64_t>(st[0]) * 2};
+  const uint32_t b[4] = {static_cast<uint32_t>(box), 1, static_cast<uint32_t>(kC), 1};
+  return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t, d, s, b, swizzle);
+}
 
 // What the forward keeps for a backward (T, P, S0, E); without one only T and P, in the workspace.
 size_t carve_fwd(Buffers* w, char* base, int64_t slots, int64_t H, int64_t V, int64_t K, bool keep) {
@@ -78,6 +116,7 @@ int check(const A* a, const char* what, Shape* s) {
                 static_cast<long long>(s->nseq), static_cast<long long>(s->batch));
   if (a->dtype != EMA_DTYPE_F32 && a->dtype != EMA_DTYPE_BF16 && a->dtype != EMA_DTYPE_F16)
     return fail(EMA_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", what, a->dtype);
+  if ((a->flags & ~DELTA_FP32_PRODUCTS) != 0) return fail(EMA_ERR_INVALID_ARGUMENT, "%s: unknown flags", what);
   if ((s->K != 64 && s->K != 128) || s->V % 8 != 0 || s->V > 128)
     return fail(EMA_ERR_UNSUPPORTED, "%s: dstate 64 or 128, headdim a multiple of 8 up to 128", what);
   if (s->H > 65535 || s->nseq > 65535 || s->seqlen > 1073741824 || slots_of(*s) > 16777216)
@@ -113,18 +152,28 @@ Params params(const A* a, const Shape& s) {
 using namespace emab::delta;
 
 extern "C" EMA_API size_t delta_saved_bytes(int64_t batch, int64_t seqlen, int64_t nseq, int64_t nheads, int64_t headdim,
-                                            int64_t dstate, int64_t ngroups, int32_t dtype) {
+                                            int64_t dstate, int64_t ngroups, int32_t dtype, int32_t flags) {
   if (batch < 0 || seqlen < 0 || nseq < 0 || nheads <= 0 || headdim <= 0 || dstate <= 0) return 0;
+  const int64_t n = slots_bound(batch, seqlen, nseq);
+  if (on_tensor_cores(dtype, seqlen, flags)) {
+    TcBuffers t{};
+    return carve_tc_fwd(&t, nullptr, n, nheads, headdim, dstate, true);
+  }
   Buffers w{};
-  return carve_fwd(&w, nullptr, slots_bound(batch, seqlen, nseq), nheads, headdim, dstate, true);
+  return carve_fwd(&w, nullptr, n, nheads, headdim, dstate, true);
 }
 
 extern "C" EMA_API size_t delta_workspace_bytes(int64_t batch, int64_t seqlen, int64_t nseq, int64_t nheads,
                                                 int64_t headdim, int64_t dstate, int64_t ngroups, int32_t dtype,
-                                                int32_t backward) {
+                                                int32_t flags, int32_t backward) {
   if (batch < 0 || seqlen < 0 || nseq < 0 || nheads <= 0 || headdim <= 0 || dstate <= 0) return 0;
   Buffers w{};
   const int64_t n = slots_bound(batch, seqlen, nseq);
+  if (on_tensor_cores(dtype, seqlen, flags)) {
+    TcBuffers t{};
+    return backward ? carve_tc_bwd(&t, nullptr, n, nheads, headdim, dstate)
+                    : carve_tc_fwd(&t, nullptr, n, nheads, headdim, dstate, false);
+  }
   return backward ? carve_bwd(&w, nullptr, n, nheads, headdim, dstate)
                   : carve_fwd(&w, nullptr, n, nheads, headdim, dstate, false);
 }
@@ -148,6 +197,26 @@ extern "C" EMA_API int delta_fwd_launch(const DeltaFwdArgs* a, void* stream) {
   Buffers w{};
   const bool keep = a->saved != nullptr;
   void* base = keep ? a->saved : a->workspace;
+  if (on_tensor_cores(a->dtype, s.seqlen, a->flags)) {
+    TcBuffers t{};
+    const size_t need = carve_tc_fwd(&t, static_cast<char*>(base), p.slots, s.H, s.V, s.K, keep);
+    if (base == nullptr || (keep ? a->saved_bytes : a->workspace_bytes) < need ||
+        reinterpret_cast<uintptr_t>(base) % 256 != 0)
+      return fail(EMA_ERR_WORKSPACE, "delta_fwd: needs %zu bytes, 256-byte aligned, of %s", need,
+                  keep ? "saved" : "workspace");
+    CUtensorMap mk{}, mq{}, mv{};
+    int e = tile_map(&mk, a->k, a->k_stride, s.K, s.G, s.seqlen, s.batch, 64, true);
+    if (e == EMA_OK) e = tile_map(&mq, a->q, a->q_stride, s.K, s.G, s.seqlen, s.batch, 64, true);
+    if (e == EMA_OK) e = tile_map(&mv, a->v, a->v_stride, s.V, s.H, s.seqlen, s.batch, s.V, false);
+    if (e != EMA_OK) return e;
+    void* st = nullptr;
+    cudaError_t ce = cudaGetSymbolAddress(&st, g_status);
+    uint32_t* status = static_cast<uint32_t*>(st);
+    if (ce == cudaSuccess) ce = tc_prep(mk, mq, p, t, status, static_cast<cudaStream_t>(stream));
+    if (ce == cudaSuccess) ce = tc_fwd_walk(mk, mq, mv, p, t, status, static_cast<cudaStream_t>(stream));
+    if (ce != cudaSuccess) return fail(EMA_ERR_CUDA, "delta_fwd launch failed: %s", cudaGetErrorString(ce));
+    return EMA_OK;
+  }
   const size_t need = carve_fwd(&w, static_cast<char*>(base), p.slots, s.H, s.V, s.K, keep);
   if (tokens && (base == nullptr || (keep ? a->saved_bytes : a->workspace_bytes) < need ||
                  reinterpret_cast<uintptr_t>(base) % 256 != 0))
@@ -179,6 +248,29 @@ extern "C" EMA_API int delta_bwd_launch(const DeltaBwdArgs* a, void* stream) {
   p.ds1 = a->d_final_states, p.ds0 = a->d_initial_states;
   p.dq = a->dq, p.vdq = view(a->dq_stride), p.dk = a->dk, p.vdk = view(a->dk_stride);
   p.dv = a->dv, p.vdv = view(a->dv_stride), p.dg = a->dg, p.dbeta = a->dbeta;
+  if (on_tensor_cores(a->dtype, s.seqlen, a->flags)) {
+    TcBuffers t{};
+    const size_t saved = carve_tc_fwd(&t, static_cast<char*>(const_cast<void*>(a->saved)), p.slots, s.H, s.V, s.K, true);
+    const size_t need = carve_tc_bwd(&t, static_cast<char*>(a->workspace), p.slots, s.H, s.V, s.K);
+    if (a->saved == nullptr || a->saved_bytes < saved || a->workspace == nullptr || a->workspace_bytes < need ||
+        reinterpret_cast<uintptr_t>(a->saved) % 256 != 0 || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0)
+      return fail(EMA_ERR_WORKSPACE, "delta_bwd: needs %zu bytes of saved and %zu of workspace, 256-byte aligned", saved,
+                  need);
+    CUtensorMap mk{}, mq{}, mo{}, mdv{};
+    int e = tile_map(&mk, a->k, a->k_stride, s.K, s.G, s.seqlen, s.batch, 64, true);
+    if (e == EMA_OK) e = tile_map(&mq, a->q, a->q_stride, s.K, s.G, s.seqlen, s.batch, 64, true);
+    if (e == EMA_OK) e = tile_map(&mo, a->dout, a->dout_stride, s.V, s.H, s.seqlen, s.batch, 64, true);
+    if (e == EMA_OK) e = tile_map(&mdv, a->dv, a->dv_stride, s.V, s.H, s.seqlen, s.batch, 64, true);
+    if (e != EMA_OK) return e;
+    cudaStream_t stm = static_cast<cudaStream_t>(stream);
+    void* st = nullptr;
+    cudaError_t ce = cudaGetSymbolAddress(&st, g_status);
+    uint32_t* status = static_cast<uint32_t*>(st);
+    if (ce == cudaSuccess) ce = tc_bwd_walk(mk, mq, mo, p, t, status, stm);
+    if (ce == cudaSuccess) ce = tc_grads(mk, mq, mo, mdv, p, t, status, stm);
+    if (ce != cudaSuccess) return fail(EMA_ERR_CUDA, "delta_bwd launch failed: %s", cudaGetErrorString(ce));
+    return EMA_OK;
+  }
   Buffers w{};
   const size_t saved = carve_fwd(&w, static_cast<char*>(const_cast<void*>(a->saved)), p.slots, s.H, s.V, s.K, true);
   const size_t need = carve_bwd(&w, static_cast<char*>(a->workspace), p.slots, s.H, s.V, s.K);
@@ -189,5 +281,18 @@ extern "C" EMA_API int delta_bwd_launch(const DeltaBwdArgs* a, void* stream) {
                 need);
   const cudaError_t e = simt_bwd(p, w, a->dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(EMA_ERR_CUDA, "delta_bwd launch failed: %s", cudaGetErrorString(e));
+  return EMA_OK;
+}
+
+extern "C" EMA_API int delta_device_status(uint32_t* status, int clear, void* stream) {
+  if (status == nullptr) return fail(EMA_ERR_INVALID_ARGUMENT, "delta_device_status: NULL");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint32_t v = 0, z = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_status, 4, 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbolAsync(g_status, &z, 4, 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess && clear) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail(EMA_ERR_CUDA, "delta_device_status: %s", cudaGetErrorString(e));
+  *status = v;
   return EMA_OK;
 }

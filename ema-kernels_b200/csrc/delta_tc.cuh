@@ -1,0 +1,113 @@
+// Shared pieces of the tensor-core (tcgen05) kernels of the gated delta rule: the buffers between them as
+// operand images, and 32-bit precision out of bf16 products.
+//
+// Precision.  States, gate gradients and every other fp32 output have to be good to fp32's own order, so a product's
+// operand that is not bf16 by nature (T, X, U, S, dX, dS) enters as a pair of bf16: hi = bf16(x), lo = bf16(x - hi),
+// x = hi + lo to 2^-17.  A bf16 tensor times a pair is two MMAs, a pair times a pair three (lo lo is dropped at
+// 2^-18).  Only what ends in a bf16 output alone (o's two terms, dq and dk) uses the hi parts.
+//
+// Images.  What one kernel leaves for the next as an MMA operand lies in global memory as the 128-byte swizzled
+// tile that shared memory wants (rows of 64 bf16, 16-byte chunk c of row r at c ^ (r % 8)), so that a plain
+// bulk copy stages it and the writing thread stores whole 16-byte chunks of its own row:
+//   T, P   64 x 64, row = token i, column = token j: hi, lo (8 KB each)
+//   E, dX  row = value channel, column = token: hi, lo
+//   S, dS  row = value channel, one region per 64 state columns: hi regions, lo regions
+#pragma once
+
+#include "delta_common.cuh"
+#include "tc_common.cuh"
+
+namespace emab {
+namespace delta {
+
+constexpr int kTile = kC * 128;  // bytes of a 64-row, 128-byte-row region
+// gate record of a (chunk, head): -exp(b_i), beta_i exp(b_end - b_i), beta_i, b_i (64 each), exp(b_end)
+constexpr int kGateFloats = 320;
+constexpr uint32_t kStatusTmem = 0x200u;  // device status: a block that owns all of tensor memory did not get base 0
+constexpr int kGateE = 0, kGateW = 64, kGateBeta = 128, kGateB = 192, kGateEnd = 256;
+
+struct TcBuffers {
+  float* gates;      // kGateFloats per (slot, head)
+  char* T;           // hi, lo
+  char* P;           // hi, lo
+  char* S;           // state entering the chunk: hi, lo (null: not kept)
+  char* E;           // hi, lo (null: not kept)
+  char* dS;          // gradient of the state at the chunk's end: hi, lo
+  char* dX;          // lo
+};
+
+__host__ __device__ inline int pad_channels(int V) { return V <= 64 ? 64 : 128; }
+__host__ __device__ inline size_t state_image(int V, int K) { return static_cast<size_t>(pad_channels(V)) * K * 2; }
+__host__ __device__ inline size_t token_image(int V) { return static_cast<size_t>(pad_channels(V)) * 128; }
+
+// bf16 pair (x, y) -> packed hi and packed lo.
+__device__ __forceinline__ void split2(float2 v, uint32_t& hi, uint32_t& lo) {
+  hi = pack_pair<__nv_bfloat16>(v);
+  lo = pack_pair<__nv_bfloat16>(f2_fma(cvt_pair<__nv_bfloat16>(hi), make_float2(-1.f, -1.f), v));
+}
+
+// D[tmem] (+)= A[tmem] B^T for one K = 16 step: A's 16 columns are 8 packed 32-bit tensor-memory columns.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+
+// One lane of a converged warp.  MMA issue stands under this and takes warp-uniform operands (descriptors from the loop
+// counter and the shared-memory base, tensor-memory addresses from a base of zero): operands the compiler cannot
+// prove uniform cost a few tens of cycles each, more than the MMA they feed.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0u;
+}
+
+// 32 lanes x 16 columns of raw 32-bit words.
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// A warpgroup's share of the registers the block was launched with; all its warps call it.
+template <int N>
+__device__ __forceinline__ void set_regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Bounded wait of the chain's roles: no sleep between the polls (a poll suspends the thread in hardware for a
+// while by itself), since every nanosecond after the phase completes is on the chain, and few instructions: the
+// kernels' loops are long and instruction fetches from beyond the caches cost more than the waits.
+constexpr long long kWaitLimitCycles = 2000000000ll;  // about a second
+__device__ __forceinline__ bool chain_wait(uint64_t* bar, uint32_t phase, uint32_t* status, volatile uint32_t* fail) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, phase)) {
+    if (clock64() - t0 > kWaitLimitCycles) {
+      atomicOr(status, kStatusTmaTimeout);
+      *fail = 1u;
+      break;
+    }
+  }
+  return *fail == 0u;
+}
+
+// Zero rows [from, 64) of `regions` 64-row regions `stride` bytes apart (one warp).
+__device__ __forceinline__ void zero_rows(unsigned char* base, int regions, int stride, int from) {
+  const int n = (kC - from) * 8;
+  for (int r = 0; r < regions; ++r)
+    for (int i = threadIdx.x & 31; i < n; i += 32)
+      *reinterpret_cast<uint4*>(base + r * stride + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+}  // namespace delta
+}  // namespace emab

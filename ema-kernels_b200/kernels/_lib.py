@@ -126,6 +126,8 @@ class EmaSpanFoldArgs(ctypes.Structure):
     ]
 
 
+DELTA_FP32_PRODUCTS = 1
+
 SPAN_EXCHANGE_MAX_RANKS = 8
 P2P_HANDLE_BYTES = 64
 
@@ -161,6 +163,7 @@ class DeltaFwdArgs(ctypes.Structure):
         ("final_states", _ptr),
         ("workspace", _ptr), ("workspace_bytes", ctypes.c_size_t),
         ("saved", _ptr), ("saved_bytes", ctypes.c_size_t),
+        ("flags", _i32), ("reserved", _i32),
     ]
 
 
@@ -181,6 +184,7 @@ class DeltaBwdArgs(ctypes.Structure):
         ("dv", _ptr), ("dv_stride", _i64 * 3),
         ("dg", _ptr), ("dbeta", _ptr), ("d_initial_states", _ptr),
         ("workspace", _ptr), ("workspace_bytes", ctypes.c_size_t),
+        ("flags", _i32), ("reserved", _i32),
     ]
 
 
@@ -280,10 +284,12 @@ for _name, _args in (("delta_fwd_launch", DeltaFwdArgs), ("delta_bwd_launch", De
                      ("residual_norm_bwd_launch", ResidualNormArgs)):
     getattr(lib, _name).restype = ctypes.c_int
     getattr(lib, _name).argtypes = [ctypes.POINTER(_args), _ptr]
+lib.delta_device_status.restype = ctypes.c_int
+lib.delta_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), ctypes.c_int, _ptr]
 lib.delta_workspace_bytes.restype = ctypes.c_size_t
-lib.delta_workspace_bytes.argtypes = [_i64] * 7 + [_i32] * 2
+lib.delta_workspace_bytes.argtypes = [_i64] * 7 + [_i32] * 3
 lib.delta_saved_bytes.restype = ctypes.c_size_t
-lib.delta_saved_bytes.argtypes = [_i64] * 7 + [_i32]
+lib.delta_saved_bytes.argtypes = [_i64] * 7 + [_i32] * 2
 lib.block_norm_workspace_bytes.restype = ctypes.c_size_t
 lib.block_norm_workspace_bytes.argtypes = [_i64] * 3
 lib.ema_last_error.restype = ctypes.c_char_p

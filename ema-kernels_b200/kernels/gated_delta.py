@@ -61,7 +61,7 @@ def _rows(t):
     """t itself where its rows can be addressed as they are: unit last stride, 16-byte steps and base."""
     es = t.element_size()
     steps = [s for s, n in zip(t.stride()[:3], t.shape) if n > 1]
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any((s * es) % 16 for s in steps):
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s <= 0 or (s * es) % 16 for s in steps):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -80,7 +80,7 @@ def _set_shape(a, dims, nseq, dtype, scale):
     a.nseq, a.dtype, a.scale = nseq, _lib.DTYPE_CODES[dtype], scale
 
 
-def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, want_final, save):
+def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final, save):
     """One forward launch: (o, final states or None, what a backward needs or None)."""
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
@@ -93,7 +93,8 @@ def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, want_final, 
     final = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_final else None
     a = _lib.DeltaFwdArgs()
     _set_shape(a, dims, nseq, v.dtype, scale)
-    size = (b, length, nseq, H, V, K, G, a.dtype)
+    a.flags = flags
+    size = (b, length, nseq, H, V, K, G, a.dtype, flags)
     nbytes = _lib.lib.delta_saved_bytes(*size) if save else _lib.lib.delta_workspace_bytes(*size, 0)
     buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     a.q, a.q_stride, a.k, a.k_stride = q.data_ptr(), _strides(q), k.data_ptr(), _strides(k)
@@ -110,7 +111,7 @@ def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, want_final, 
     return o, final, buf if save else None
 
 
-def _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial):
+def _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, flags, want_d_initial):
     """One backward launch: (dq, dk, dv, dg, dbeta, d initial states or None); dg, dbeta fp32."""
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
@@ -124,7 +125,8 @@ def _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_i
     ds0 = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_d_initial else None
     a = _lib.DeltaBwdArgs()
     _set_shape(a, (b, length, H, V, G, K), nseq, v.dtype, scale)
-    nbytes = _lib.lib.delta_workspace_bytes(b, length, nseq, H, V, K, G, a.dtype, 1)
+    a.flags = flags
+    nbytes = _lib.lib.delta_workspace_bytes(b, length, nseq, H, V, K, G, a.dtype, flags, 1)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     for name, t in (("q", q), ("k", k), ("v", v), ("dout", do), ("dq", dq), ("dk", dk), ("dv", dv)):
         setattr(a, name, t.data_ptr())
@@ -147,18 +149,18 @@ def _empty0(like):
 
 @torch.library.custom_op("ema_b200::delta_fwd", mutates_args=(), device_types="cuda")
 def _delta_fwd_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
-                  initial_states: Optional[torch.Tensor], cu_seqlens: Optional[torch.Tensor],
-                  scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                  initial_states: Optional[torch.Tensor], cu_seqlens: Optional[torch.Tensor], scale: float,
+                  flags: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(o, the final states, what the backward reads)."""
-    return _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, True, True)
+    return _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, True, True)
 
 
 @_delta_fwd_op.register_fake
-def _(q, k, v, g, beta, initial_states, cu_seqlens, scale):
+def _(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags=0):
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
     nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    nbytes = _lib.lib.delta_saved_bytes(b, length, nseq, H, V, K, G, _lib.DTYPE_CODES[v.dtype])
+    nbytes = _lib.lib.delta_saved_bytes(b, length, nseq, H, V, K, G, _lib.DTYPE_CODES[v.dtype], flags)
     return (v.new_empty((b, length, H, V)), v.new_empty((nseq, H, V, K), dtype=torch.float32),
             v.new_empty((nbytes,), dtype=torch.uint8))
 
@@ -166,16 +168,16 @@ def _(q, k, v, g, beta, initial_states, cu_seqlens, scale):
 @torch.library.custom_op("ema_b200::delta_bwd", mutates_args=(), device_types="cuda")
 def _delta_bwd_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                   cu_seqlens: Optional[torch.Tensor], saved: torch.Tensor, do: torch.Tensor,
-                  d_final: Optional[torch.Tensor], scale: float,
+                  d_final: Optional[torch.Tensor], scale: float, flags: int,
                   want_d_initial: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
                                                  torch.Tensor]:
     """(dq, dk, dv, dg, dbeta, d initial states), the last empty when not wanted."""
-    *grads, ds0 = _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial)
+    *grads, ds0 = _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, flags, want_d_initial)
     return (*grads, ds0 if ds0 is not None else _empty0(v))
 
 
 @_delta_bwd_op.register_fake
-def _(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial):
+def _(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, flags, want_d_initial):
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
     nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
@@ -186,9 +188,9 @@ def _(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, want_d_initial):
 
 
 def _setup(ctx, inputs, output):
-    q, k, v, g, beta, initial_states, cu_seqlens, scale = inputs
+    q, k, v, g, beta, initial_states, cu_seqlens, scale, flags = inputs
     ctx.save_for_backward(q, k, v, g, beta, cu_seqlens, output[2])
-    ctx.scale = scale
+    ctx.scale, ctx.flags = scale, flags
     ctx.d_initial = initial_states is not None and ctx.needs_input_grad[5]
     ctx.initial_dtype = None if initial_states is None else initial_states.dtype
     ctx.set_materialize_grads(False)
@@ -197,19 +199,20 @@ def _setup(ctx, inputs, output):
 def _backward(ctx, do, d_final, _d_saved):
     q, k, v, g, beta, cu, saved = ctx.saved_tensors
     if do is None and d_final is None:
-        return (None,) * 8
+        return (None,) * 9
     if do is None:
         do = torch.zeros_like(v)
     dq, dk, dv, dg, dbeta, ds0 = torch.ops.ema_b200.delta_bwd(q, k, v, g, beta, cu, saved, do, d_final, ctx.scale,
-                                                              ctx.d_initial)
+                                                              ctx.flags, ctx.d_initial)
     return (dq, dk, dv, dg.to(g.dtype), dbeta.to(beta.dtype), ds0.to(ctx.initial_dtype) if ctx.d_initial else None,
-            None, None)
+            None, None, None)
 
 
 torch.library.register_autograd("ema_b200::delta_fwd", _backward, setup_context=_setup)
 
 
-def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_final_states=False, cu_seqlens=None):
+def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_final_states=False, cu_seqlens=None,
+                     fp32_products=False):
     """o (batch, seqlen, nheads, headdim), or (o, final states) with ``return_final_states``.
 
     g is the log decay (not positive in a decaying layer; at or below -100 the state is dropped), beta the write
@@ -219,7 +222,10 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
     (its final state is its initial one); tokens outside every sequence give zeros.
 
     Gradients: q, k, v, g, beta and initial_states; those of a group's q and k sum over its heads.  The states,
-    all sums and both gate gradients are fp32."""
+    all sums and both gate gradients are fp32.  bf16 calls run on the tensor cores with their 32-bit operands as
+    pairs of bf16: 2^-17 of each, some 5e-6 of a state or gate gradient.  Where keys repeat and beta is near one,
+    the gate gradients are small differences of large terms and keep fewer digits; ``fp32_products`` then gives
+    those of fp32 arithmetic, at about twenty times the time.  fp16 and fp32 calls are always fp32 products."""
     b, length, H, V, G, K = _check(q, k, v, g, beta, "gated_delta_rule")
     _check_headdim(V, 128, "gated_delta_rule")
     nseq = b
@@ -237,12 +243,15 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
             raise ValueError(f"gated_delta_rule: initial_states must be {(nseq, H, V, K)} on v's device, got "
                              f"{tuple(initial_states.shape)}")
     scale = K ** -0.5 if scale is None else float(scale)
+    flags = _lib.DELTA_FP32_PRODUCTS if fp32_products else 0
     wants = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states))
     if wants or torch.compiler.is_compiling():
-        o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale)
+        o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale,
+                                                   flags)
     else:
-        o, final, _ = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, return_final_states, False)
+        o, final, _ = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, return_final_states,
+                                 False)
     return (o, final) if return_final_states else o
 
 

@@ -26,6 +26,10 @@
 extern "C" {
 #endif
 
+/* bf16 calls run on the tensor cores, their 32-bit operands as pairs of bf16 (2^-17 of each); with this flag
+ * their products are fp32 on the CUDA cores, as those of fp16 and fp32 calls always are. */
+#define DELTA_FP32_PRODUCTS 1
+
 typedef struct DeltaFwdArgs {
   int64_t batch, seqlen, nheads, headdim, dstate, ngroups;
   int64_t nseq;                  /* sequences: batch without cu_seqlens */
@@ -42,6 +46,8 @@ typedef struct DeltaFwdArgs {
   float* final_states;           /* or NULL */
   void* workspace; size_t workspace_bytes;  /* delta_workspace_bytes(.., 0) */
   void* saved; size_t saved_bytes;          /* delta_saved_bytes(): kept for the backward; NULL without one */
+  int32_t flags;                 /* DELTA_FP32_PRODUCTS or 0; the same for the sizes, the forward and the backward */
+  int32_t reserved;
 } DeltaFwdArgs;
 
 typedef struct DeltaBwdArgs {
@@ -65,6 +71,8 @@ typedef struct DeltaBwdArgs {
   float* dbeta;
   float* d_initial_states;       /* or NULL */
   void* workspace; size_t workspace_bytes;  /* delta_workspace_bytes(.., 1) */
+  int32_t flags;
+  int32_t reserved;
 } DeltaBwdArgs;
 
 /* The recurrent form: `tokens` tokens of every row on a cache of states, updated in place.  Row b works on
@@ -86,12 +94,15 @@ typedef struct DeltaStepArgs {
 
 /* Bytes of scratch (contents need not be initialised) and of what the forward keeps for the backward. */
 EMA_API size_t delta_workspace_bytes(int64_t batch, int64_t seqlen, int64_t nseq, int64_t nheads, int64_t headdim,
-                                     int64_t dstate, int64_t ngroups, int32_t dtype, int32_t backward);
+                                     int64_t dstate, int64_t ngroups, int32_t dtype, int32_t flags, int32_t backward);
 EMA_API size_t delta_saved_bytes(int64_t batch, int64_t seqlen, int64_t nseq, int64_t nheads, int64_t headdim,
-                                 int64_t dstate, int64_t ngroups, int32_t dtype);
+                                 int64_t dstate, int64_t ngroups, int32_t dtype, int32_t flags);
 EMA_API int delta_fwd_launch(const DeltaFwdArgs* args, void* stream);
 EMA_API int delta_bwd_launch(const DeltaBwdArgs* args, void* stream);
 EMA_API int delta_step_launch(const DeltaStepArgs* args, void* stream);
+/* Error word of the chunked kernels (0: none; 2: a bounded wait on the device timed out and results are
+ * invalid), read on `stream` after the work queued before it; zeroed afterwards when `clear` is non-zero. */
+EMA_API int delta_device_status(uint32_t* status, int clear, void* stream);
 
 #ifdef __cplusplus
 }

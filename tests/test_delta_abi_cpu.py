@@ -57,7 +57,7 @@ def _delta(cls, **kw):
 # (1: invalid argument, 2: unsupported, 3: workspace; every pointer is checked before anything is launched)
 @pytest.mark.parametrize("kw,code", [(dict(ngroups=3), 1), (dict(headdim=12), 2), (dict(headdim=136), 2),
                                      (dict(dstate=96), 2), (dict(dtype=7), 1), (dict(nseq=3), 1), (dict(batch=-1), 1),
-                                     (dict(), 1), (dict(nheads=131072), 2)])
+                                     (dict(), 1), (dict(nheads=131072), 2), (dict(flags=2), 1)])
 def test_sequence_launchers_refuse(kw, code):
     from kernels import _lib
     for name in ("delta_fwd", "delta_bwd"):
@@ -120,7 +120,7 @@ def test_residual_norm_refuses():
 def test_buffer_sizes_cover_packed_calls():
     """A packed call may use a slot per 64 tokens and one per sequence; sizes grow with both."""
     from kernels import _lib
-    size = lambda L, n: _lib.lib.delta_saved_bytes(1, L, n, 2, 64, 64, 1, 1)  # noqa: E731
+    size = lambda L, n: _lib.lib.delta_saved_bytes(1, L, n, 2, 64, 64, 1, 1, 0)  # noqa: E731
     assert size(640, 1) < size(640, 5) and size(640, 5) < size(6400, 5)
 
 

@@ -29,7 +29,7 @@ def _round(x, dt):
     return torch.from_numpy(x).to(dt).double().numpy()
 
 
-def _case(lens, G, H, K, V, dt, seed, states, g_edit=None, packed=False):
+def _case(lens, G, H, K, V, dt, seed, states, g_edit=None, packed=False, **kw):
     """Runs forward + backward on the GPU and the oracle sequence by sequence; returns {name: (got, want)}."""
     from kernels.gated_delta import gated_delta_rule
     n, scale = len(lens), K ** -0.5
@@ -49,7 +49,7 @@ def _case(lens, G, H, K, V, dt, seed, states, g_edit=None, packed=False):
         x.requires_grad_()
     cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), device=DEV, dtype=torch.int32) if packed else None
     o, fin = gated_delta_rule(q, k, v, g, beta, scale=scale, initial_states=leaves[5] if states else None,
-                              return_final_states=True, cu_seqlens=cu)
+                              return_final_states=True, cu_seqlens=cu, **kw)
     outs, douts = [o], [do]
     if states:
         outs, douts = [o, fin], [do, torch.from_numpy(d1).to(DEV)]
@@ -58,7 +58,7 @@ def _case(lens, G, H, K, V, dt, seed, states, g_edit=None, packed=False):
     # the same forward without a graph takes the buffers of inference
     with torch.no_grad():
         o2, fin2 = gated_delta_rule(q, k, v, g, beta, scale=scale, initial_states=leaves[5] if states else None,
-                                    return_final_states=True, cu_seqlens=cu)
+                                    return_final_states=True, cu_seqlens=cu, **kw)
     assert torch.equal(o, o2) and torch.equal(fin, fin2)
     want = {m: [] for m in ("o", "final", "dq", "dk", "dv", "dg", "dbeta", "ds0")}
     for i, x in enumerate(per):
@@ -128,7 +128,22 @@ def test_repeated_keys(dt):
         x[1][:] = x[1][:1]
         x[4][:] = 0.98
         x[3][:] = -1e-3
-    _hold(_case([130], 1, 2, 128, 64, dt, seed=13, states=False, g_edit=edit), dt)
+    _hold(_case([130], 1, 2, 128, 64, dt, seed=13, states=False, g_edit=edit, fp32_products=True), dt)
+
+
+def test_repeated_keys_on_operand_pairs():
+    """The same on the tensor cores.  Their operand pairs hold 2^-17 of a value where fp32 holds 2^-24, so the gate
+    gradients, differences of sums of up to 32 x 32 (dg) and 64 (dbeta) products of the size scale |do| |v|, may be off
+    by 2^-17 of the root of the sum of squares of those products; everything else holds its tolerance."""
+    def edit(x):
+        x[1][:] = x[1][:1]
+        x[4][:] = 0.98
+        x[3][:] = -1e-3
+    res = _case([130], 1, 2, 128, 64, torch.bfloat16, seed=13, states=False, g_edit=edit)
+    for m, terms in (("dg", 32), ("dbeta", 8)):
+        got, want = res.pop(m)
+        assert np.linalg.norm(got.double().cpu().numpy() - want) <= 2.0 ** -17 * terms * res["size"], m
+    _hold(res, torch.bfloat16)
 
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
@@ -293,3 +308,13 @@ def test_refusals():
     a[2].requires_grad_()
     with pytest.raises(ValueError):
         gated_delta_step(*a, st)
+
+
+def test_device_status_is_clear():
+    """No bounded wait of the tensor-core kernels ran out in any of the calls above."""
+    import ctypes
+
+    from kernels import _lib
+    word = ctypes.c_uint32(0)
+    _lib.check(_lib.lib.delta_device_status(ctypes.byref(word), 1, _lib.stream_ptr(torch.device(DEV))), "status")
+    assert word.value == 0
