@@ -3,12 +3,11 @@
 // One block per (sequence, head) carries dS, the gradient of the state, with a tensor-memory lane per value channel as
 // in the forward walk, whose mirror it is:
 //
-//   Z = dS K^t,  Y = dO^t P  ->  W = beta Y + (beta w) Z  ->  dX = W T  ->  dS = exp(b_end) dS + dO~ Q - (exp(b) dX) K
+//   Z = dS K^t,  Y = dO^t P  ->  W = beta Y + (beta w) Z  ->  dX = W + W (T - I)  ->  dS = exp(b_end) dS + dO~ Q - (exp(b) dX) K
 //
 // with w_j = exp(b_end - b_j) and dO~_i = scale exp(b_i) dO_i.  W, dX and dS are the chain; Y (from P and dO as they
 // lie in shared memory) and dO~ Q are ready before it needs them.  Operands that are not bf16 by nature are hi + lo
-// pairs (delta_tc.cuh).  dv = dX; what the gradient kernel needs besides is left as images: dS at
-// every chunk's end (hi, lo) and dX's lo part (its hi part is dv).
+// pairs (delta_tc.cuh), dO~, whose rounding stays in dS, three pieces.  dv = dX; for the gradient kernel dS at every chunk's end and dX are left as fp32 images.
 //
 // Bound: the chain's latency, as in the forward walk (three dependent MMA groups of about 900, 750 and 950 cycles
 // with their hand-overs, and an epilogue after each).  Roles: warps 0-7 the chain's epilogues, warps 8-11 dO~ and the
@@ -37,10 +36,10 @@ constexpr int kReg = 128 * 128;  // 64 query rows, then 64 key rows of 64 column
 constexpr uint32_t cZ = 0;     // Z; then W T hi
 constexpr uint32_t cY = 64;    // Y; then W T lo
 constexpr uint32_t cW = 128;   // W hi, lo; then -exp(b) dX hi, lo (32 columns each)
-constexpr uint32_t cO = 192;   // dO~ hi, lo
 constexpr uint32_t cDS = 256;
 constexpr uint32_t cDh = 384;  // dS hi (K / 2 columns)
 constexpr uint32_t cDl = 448;  // dS lo
+constexpr uint32_t cO = 384;   // dO~ hi, mid, lo (32 columns each), once Z has read dS
 
 struct Bars {
   uint64_t full[kStages], empty[kStages];
@@ -207,6 +206,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cO + 8 * s, dqn + nstep(s), idK, s > 0);
 #pragma unroll
           for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cO + 32 + 8 * s, dqn + nstep(s), idK, true);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cO + 64 + 8 * s, dqn + nstep(s), idK, true);
         }
         __syncwarp();
         ok = wait(&bar.wx, r & 1);
@@ -240,12 +241,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* gate = reinterpret_cast<const float*>(base + St::oG);
       const int have = min(kC, q.len - c * kC);
       if (!wait(&bar.full[st], (r / kStages) & 1)) break;
-      if (r > 0 && !wait(&bar.ds, (r - 1) & 1)) break;  // the last step's dO~ has been read
+      if (!wait(&bar.z, r & 1)) break;
+      tc::fence_after_sync();
       const unsigned char* src = base + St::oO + (row >> 6) * kTile;
       const uint32_t col = (row & 63) * 2;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        uint32_t hi[16], lo[16];
+        uint32_t hi[16], mid[16], lo[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = 32 * g + 2 * i;
@@ -255,10 +257,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           v.y = to_f32(*reinterpret_cast<const __nv_bfloat16*>(src + (t + 1) * 128 + (col ^ (((t + 1) & 7) << 4))));
           v.x = (live && t < have) ? v.x * (-p.scale * e.x) : 0.f;
           v.y = (live && t + 1 < have) ? v.y * (-p.scale * e.y) : 0.f;
-          split2(v, hi[i], lo[i]);
+          split3(v, hi[i], mid[i], lo[i]);
         }
         tmem_st16u(tb + tl + cO + 16 * g, hi);
-        tmem_st16u(tb + tl + cO + 32 + 16 * g, lo);
+        tmem_st16u(tb + tl + cO + 32 + 16 * g, mid);
+        tmem_st16u(tb + tl + cO + 64 + 16 * g, lo);
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
@@ -306,7 +309,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* gate = reinterpret_cast<const float*>(base + St::oG);
       const long long ch = static_cast<long long>(q.slot + c) * p.H + h;
       {  // dS as hi / lo operand columns, and as the image of this chunk's end
-        char* img = w.dS + ch * 2 * state_image(p.V, K) + (hf * KC / 64) * VP * 128;
+        if (row < VP) {
+          float* img = w.dS + ch * state_image(p.V, K);
+#pragma unroll
+          for (int i = 0; i < KC / 4; ++i)
+            *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
+                make_float4(D[2 * i].x, D[2 * i].y, D[2 * i + 1].x, D[2 * i + 1].y);
+        }
 #pragma unroll
         for (int g = 0; g < KC / 32; ++g) {
           uint32_t hi[16], lo[16];
@@ -314,21 +323,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 16; ++i) split2(D[16 * g + i], hi[i], lo[i]);
           tmem_st16u(tb + tl + cDh + hf * (KC / 2) + 16 * g, hi);
           tmem_st16u(tb + tl + cDl + hf * (KC / 2) + 16 * g, lo);
-          if (row < VP) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t at = tc::chunk_off(row, (hf * KC % 64) / 8 + 4 * g + i);
-              *reinterpret_cast<uint4*>(img + at) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-              *reinterpret_cast<uint4*>(img + state_image(p.V, K) + at) =
-                  make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-            }
-          }
         }
         tc::tmem_wait_st();
       }
       arrive(&bar.s);
       if (!wait(&bar.full[st], (r / kStages) & 1) || !wait(&bar.z, r & 1)) break;
       tc::fence_after_sync();
+      float2 x[16];  // W, then dX
       {  // W = beta Y + (beta w) Z
         float a[2][16], b[2][16];
         uint32_t hi[16], lo[16];
@@ -341,7 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 16; ++i) {
           const float2 be = *reinterpret_cast<const float2*>(gate + kGateBeta + 32 * hf + 2 * i);
           const float2 bw = *reinterpret_cast<const float2*>(gate + kGateW + 32 * hf + 2 * i);
-          split2(f2_fma(bw, pair(a, i), f2_mul(be, pair(b, i))), hi[i], lo[i]);
+          x[i] = f2_fma(bw, pair(a, i), f2_mul(be, pair(b, i)));
+          split2(x[i], hi[i], lo[i]);
         }
         tmem_st16u(tb + tl + cW + 16 * hf, hi);
         tmem_st16u(tb + tl + cW + 32 + 16 * hf, lo);
@@ -351,7 +353,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait(&bar.dx, r & 1)) break;
       tc::fence_after_sync();
       {
-        float2 x[16];  // dX
         uint32_t hi[16], lo[16];
         {
           float a[2][16], b[2][16];
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            x[i] = f2_add(pair(a, i), pair(b, i));
+            x[i] = f2_add(x[i], f2_add(pair(a, i), pair(b, i)));
             split2(f2_mul(*reinterpret_cast<const float2*>(gate + kGateE + 32 * hf + 2 * i), x[i]), hi[i], lo[i]);
           }
         }
@@ -370,17 +371,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st16u(tb + tl + cW + 32 + 16 * hf, lo);
         tc::tmem_wait_st();
         arrive(&bar.wx);
-        // while the state product runs: dX's lo image, its hi part over dO's tile
+        // while the state product runs: dX's image, dv over dO's tile
         if (!wait(&bar.dot, r & 1)) break;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) split2(x[i], hi[i], lo[i]);
         if (row < VP) {
-          char* img = w.dX + ch * token_image(p.V);
+          float* img = w.dX + ch * token_image(p.V);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(img + tc::chunk_off(row, 4 * hf + i)) =
-                make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(img + image_at(VP, row, 8 * hf + i)) =
+                make_float4(x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y);
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) hi[i] = pack_pair<__nv_bfloat16>(x[i]);
         if (live) {
           uint16_t* so = reinterpret_cast<uint16_t*>(base + St::oO) + 32 * hf * p.V + row;
 #pragma unroll

@@ -3,12 +3,12 @@
 // One block per (sequence, head) carries the state through the chunks.  Everything is held transposed: a
 // tensor-memory lane is a value channel, so the chain of products
 //
-//   KS = S K^t  ->  X = V^t - exp(b) KS  ->  E = X T^t  ->  U = beta E  ->  S = exp(b_end) S + (w U) K
+//   KS = S K^t  ->  X = V^t - exp(b) KS  ->  E = X + X (T - I)^t  ->  U = beta E  ->  S = exp(b_end) S + (w U) K
 //
 // is a chain of M = 128 MMAs whose left operand (S, X, U) the epilogue threads write straight back to tensor memory
 // -- no shared-memory round trip and no transpose -- and whose right operands K, Q, T, P are the tiles as
-// loaded.  Operands that are not bf16 by nature are hi + lo pairs (delta_tc.cuh): 2 products for S K^t, S Q^t and
-// the state, 3 for E and U P^t.  (o = scale exp(b) S Q^t + U P^t ends in bf16, but where keys repeat its two terms
+// loaded.  Operands that are not bf16 by nature are hi + lo pairs (delta_tc.cuh): 2 products for S K^t and S Q^t, 3
+// for E and U P^t; w U, whose rounding stays in the state, is three pieces.  (o = scale exp(b) S Q^t + U P^t ends in bf16, but where keys repeat its two terms
 // cancel: hi parts alone left it 1e-2 off there.)
 //
 // Bound: the chain's latency.  A chunk is three dependent MMA groups (about 1000, 640 and 770 cycles at dstate
@@ -32,26 +32,25 @@ constexpr int kOut = 4;                      // output warps
 constexpr int kMma = 12, kLoad = 13;         // (14 and 15 only fill their warpgroup)
 constexpr int kThreads = 16 * 32;
 // registers a thread, by warpgroup: 2 epilogue, output, MMA and loads; 4 x 128 at launch
-constexpr int kRegEpi = 168, kRegOut = 96, kRegCtl = 80;
+constexpr int kRegEpi = 160, kRegOut = 120, kRegCtl = 72;
 static_assert(2 * kRegEpi + kRegOut + kRegCtl == 4 * 128, "register split");
 constexpr int kStages = 2;
 constexpr int kReg = 128 * 128;              // 64 query rows, then 64 key rows of 64 columns
 
 // tensor-memory columns.  An MMA step with its left operand in tensor memory takes about 32 + N / 2 cycles here, so what
 // can share one runs as N = 128: X [T hi; T lo]^t.
-constexpr uint32_t cQS = 0;
-constexpr uint32_t cKS = 64;   // K S; then X T hi^t; then U: hi and lo of tokens 0-31, hi and lo of 32-63 (16 columns each)
-constexpr uint32_t cPU = 128;  // X T lo^t; then U P^t
-constexpr uint32_t cX = 192;   // X hi, X lo; then w U hi, lo (32 columns each)
-constexpr uint32_t cDS = 256;
+constexpr uint32_t cX = 0;     // X hi, lo; then w U hi, mid, lo (32 columns each)
+constexpr uint32_t cKS = 128;  // K S; then X (T hi)^t; then U: hi and lo of tokens 0-31, hi and lo of 32-63 (16 columns each)
+constexpr uint32_t cPU = 192;  // X (T lo)^t; then U P^t
+constexpr uint32_t cDS = 256;  // Q S (64 columns), read before the state's product needs the place
 constexpr uint32_t cSh = 384;  // S hi (K / 2 columns)
 constexpr uint32_t cSl = 448;  // S lo
 
 struct Bars {
   uint64_t full[kStages], empty[kStages];
-  uint64_t ks, e, ds, pu;  // MMA groups done
+  uint64_t ks, qs, e, ds, pu;  // MMA groups done
   uint64_t s, x, wu, u;    // epilogues done: state, X, w U and U ready
-  uint64_t o;              // Q S and U P read
+  uint64_t q, o;           // Q S, U P read
   uint64_t out_sync;       // meeting of the output warps (bounded, unlike a barrier instruction)
   uint64_t drain;          // MMAs still in flight after a failed wait
   uint32_t taddr, fail;
@@ -97,7 +96,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.x, kEpi);
     mbar_init(&bar.wu, kEpi);
     mbar_init(&bar.u, kEpi);
+    mbar_init(&bar.q, kOut);
     mbar_init(&bar.o, kOut);
+    mbar_init(&bar.qs, 1);
     mbar_init(&bar.pu, 1);
     mbar_init(&bar.out_sync, kOut);
     mbar_init(&bar.drain, 1);
@@ -181,15 +182,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::mma_commit(&bar.ks);
         }
         __syncwarp();
-        if (c > 0 && !wait(&bar.o, (c - 1) & 1)) break;  // Q S and U P have been read
-        tc::fence_after_sync();
         if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < K / 16; ++s) mma_ts(tb + cQS, tb + cSh + 8 * s, dq + kstep(s), id64, s > 0);
+          for (int s = 0; s < K / 16; ++s) mma_ts(tb + cDS, tb + cSh + 8 * s, dq + kstep(s), id64, s > 0);
 #pragma unroll
-          for (int s = 0; s < K / 16; ++s) mma_ts(tb + cQS, tb + cSl + 8 * s, dq + kstep(s), id64, true);
+          for (int s = 0; s < K / 16; ++s) mma_ts(tb + cDS, tb + cSl + 8 * s, dq + kstep(s), id64, true);
+          tc::mma_commit(&bar.qs);
         }
         __syncwarp();
+        if (c > 0 && !wait(&bar.o, (c - 1) & 1)) break;  // U P has been read where X (T lo)^t goes
         if (!wait(&bar.x, c & 1)) break;
         tc::fence_after_sync();
         if (elect_one()) {
@@ -200,13 +201,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::mma_commit(&bar.e);
         }
         __syncwarp();
-        if (!wait(&bar.wu, c & 1)) break;
+        if (!wait(&bar.q, c & 1) || !wait(&bar.wu, c & 1)) break;
         tc::fence_after_sync();
         if (elect_one()) {
 #pragma unroll
           for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cX + 8 * s, dkn + nstep(s), idK, s > 0);
 #pragma unroll
           for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cX + 32 + 8 * s, dkn + nstep(s), idK, true);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cX + 64 + 8 * s, dkn + nstep(s), idK, true);
           tc::mma_commit(&bar.ds);
         }
         __syncwarp();
@@ -240,21 +243,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       unsigned char* base = smem + st * St::kBytes;
       const float* gate = reinterpret_cast<const float*>(base + St::oG);
       const int have = min(kC, q.len - c * kC);
-      if (!wait(&bar.full[st], (c / kStages) & 1) || !wait(&bar.pu, c & 1)) break;
+      if (!wait(&bar.full[st], (c / kStages) & 1) || !wait(&bar.qs, c & 1)) break;
       tc::fence_after_sync();
-      uint32_t o[32];  // token pairs
+      float2 f[32];  // token pairs
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float a[16], b[16];
-        tc::tmem_ld16(tb + tl + cQS + 16 * g, a);
-        tc::tmem_ld16(tb + tl + cPU + 16 * g, b);
+      for (int g = 0; g < 2; ++g) {
+        float a[2][16];
+        tc::tmem_ld16(tb + tl + cDS + 32 * g, a[0]);
+        tc::tmem_ld16(tb + tl + cDS + 32 * g + 16, a[1]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + 16 * g + 2 * i);
-          o[8 * g + i] = pack_pair<__nv_bfloat16>(
-              make_float2(fmaf(-p.scale * e.x, a[2 * i], b[2 * i]), fmaf(-p.scale * e.y, a[2 * i + 1], b[2 * i + 1])));
-        }
+        for (int i = 0; i < 16; ++i)
+          f[16 * g + i] = f2_mul(f2_mul(f2_bcast(-p.scale), *reinterpret_cast<const float2*>(gate + kGateE + 32 * g + 2 * i)),
+                                 pair(a, i));
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.q);
+      if (!wait(&bar.pu, c & 1)) break;
+      tc::fence_after_sync();
+      uint32_t o[32];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float a[16];
+        tc::tmem_ld16(tb + tl + cPU + 16 * g, a);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          o[8 * g + i] = pack_pair<__nv_bfloat16>(f2_add(f[8 * g + i], make_float2(a[2 * i], a[2 * i + 1])));
       }
       tc::fence_before_sync();
       __syncwarp();
@@ -309,7 +325,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the state as hi / lo operand columns, and as the image of the chunk it enters
     auto publish = [&](int c) {
       const long long ch = static_cast<long long>(q.slot + c) * p.H + h;
-      char* img = KEEP ? w.S + ch * 2 * state_image(p.V, K) + (hf * KC / 64) * VP * 128 : nullptr;
+      if (KEEP && row < VP) {
+        float* img = w.S + ch * state_image(p.V, K);
+#pragma unroll
+        for (int i = 0; i < KC / 4; ++i)
+          *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
+              make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
+      }
 #pragma unroll
       for (int g = 0; g < KC / 32; ++g) {
         uint32_t hi[16], lo[16];
@@ -317,15 +339,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 16; ++i) split2(S[16 * g + i], hi[i], lo[i]);
         tmem_st16u(tb + tl + cSh + hf * (KC / 2) + 16 * g, hi);
         tmem_st16u(tb + tl + cSl + hf * (KC / 2) + 16 * g, lo);
-        if (KEEP && row < VP) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t at = tc::chunk_off(row, (hf * KC % 64) / 8 + 4 * g + i);
-            *reinterpret_cast<uint4*>(img + at) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-            *reinterpret_cast<uint4*>(img + state_image(p.V, K) + at) =
-                make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-          }
-        }
       }
       tc::tmem_wait_st();
     };
@@ -348,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!wait(&bar.ks, c & 1)) break;
       tc::fence_after_sync();
+      float2 x[16];
       {
         float a[2][16];
         tc::tmem_ld16(tb + tl + cKS + 32 * hf, a[0]);
@@ -357,7 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + 32 * hf + 2 * i);  // -exp(b)
-          split2(f2_fma(e, pair(a, i), make_float2(v[2 * i], v[2 * i + 1])), hi[i], lo[i]);
+          x[i] = f2_fma(e, pair(a, i), make_float2(v[2 * i], v[2 * i + 1]));
+          split2(x[i], hi[i], lo[i]);
         }
         tmem_st16u(tb + tl + cX + 16 * hf, hi);
         tmem_st16u(tb + tl + cX + 32 + 16 * hf, lo);
@@ -377,15 +392,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::tmem_ld16(tb + tl + cPU + 32 * hf, b[0]);
           tc::tmem_ld16(tb + tl + cPU + 32 * hf + 16, b[1]);
           tc::tmem_wait_ld();
+          uint32_t mid[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            e[i] = f2_add(pair(a, i), pair(b, i));
-            split2(f2_mul(e[i], *reinterpret_cast<const float2*>(gate + kGateW + 32 * hf + 2 * i)), hi[i], lo[i]);
+            e[i] = f2_add(x[i], f2_add(pair(a, i), pair(b, i)));
+            split3(f2_mul(e[i], *reinterpret_cast<const float2*>(gate + kGateW + 32 * hf + 2 * i)), hi[i], mid[i], lo[i]);
           }
+          tmem_st16u(tb + tl + cX + 16 * hf, hi);
+          tmem_st16u(tb + tl + cX + 32 + 16 * hf, mid);
+          tmem_st16u(tb + tl + cX + 64 + 16 * hf, lo);
+          tc::tmem_wait_st();
         }
-        tmem_st16u(tb + tl + cX + 16 * hf, hi);
-        tmem_st16u(tb + tl + cX + 32 + 16 * hf, lo);
-        tc::tmem_wait_st();
         arrive(&bar.wu);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -397,16 +414,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         arrive(&bar.u);
         if (KEEP && row < VP) {  // E's image, while the state product runs
           const long long ch = static_cast<long long>(q.slot + c) * p.H + h;
-          char* img = w.E + ch * 2 * token_image(p.V);
+          float* img = w.E + ch * token_image(p.V);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t eh[4], el[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) split2(e[4 * i + k], eh[k], el[k]);
-            const uint32_t at = tc::chunk_off(row, 4 * hf + i);
-            *reinterpret_cast<uint4*>(img + at) = make_uint4(eh[0], eh[1], eh[2], eh[3]);
-            *reinterpret_cast<uint4*>(img + token_image(p.V) + at) = make_uint4(el[0], el[1], el[2], el[3]);
-          }
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(img + image_at(VP, row, 8 * hf + i)) =
+                make_float4(e[2 * i].x, e[2 * i].y, e[2 * i + 1].x, e[2 * i + 1].y);
         }
       }
       // S = exp(b_end) S + (w U) K

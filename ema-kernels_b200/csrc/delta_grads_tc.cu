@@ -11,13 +11,16 @@
 // and what the gates need, by transposed butterflies over the lanes of fp32 values:
 //   dbeta_j = sum of y over its column + w_j k_j . a3_j
 //   dg_t = sum over rows of (prefix of beta y up to t) + sum_{i >= t} r_i + sum_{j < t} c_j + exp(b_end) <dS1, S0>
-// dg and dbeta are fp32 results, so S0, dS1, E and dX enter as hi + lo pairs wherever they reach them (delta_tc.cuh).
-// N is a pair too where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are single bf16.
+// dg and dbeta are fp32 results, and sums that cancel: S0, dS1, E and dX enter as three bf16 pieces each, all products of
+// them down to 2^-24.  N is a pair where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are
+// single bf16.
 //
-// One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  Bound: the
-// images' bytes (S0 and dS1 are 2 x 64 KB a chunk and head at 128 x 128) and, near it, the epilogues.  Roles: warps
-// 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 <dS1, S0> and the gates' results, warp 12 the MMAs,
-// warp 13 the loads.  S0 hi and dS1 hi stay for the whole head, one more slot takes S0 lo and then dS1 lo.
+// One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  S0, dS1, E
+// and dX come as fp32 images; warps 8-11 take them through registers, sum <dS1, S0> on the way and stage the pieces, S0 and
+// dS1 in steps of 16 value channels (one MMA step) through a ring of two.  Bound: the images' bytes (S0 and dS1 are 2 x 64
+// KB a chunk and head at 128 x 128), and near it the tensor pipe (about 7500 cycles a head) and the epilogues.  Roles: warps
+// 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 staging and the gates' results, warp 12 the MMAs, warp
+// 13 the loads of Q, K, dO and dv.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -33,21 +36,22 @@ namespace {
 constexpr int kEpi = 8, kAux = 4;
 constexpr int kMma = 12, kLoad = 13;  // (14 and 15 only fill their warpgroup)
 constexpr int kThreads = 16 * 32;
-constexpr int kRegEpi = 184, kRegAux = 72, kRegCtl = 72;
+constexpr int kRegEpi = 168, kRegAux = 112, kRegCtl = 64;
 static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128, "register split");
+constexpr int kRing = 2;
 constexpr int kReg = 128 * 128;  // two 64-row tiles of 64 columns, one over the other
 
 // tensor-memory columns
 constexpr uint32_t cKQ = 0;     // [qk; kk]
-constexpr uint32_t cF = 64;     // [f; F'] of E hi, of E lo, then of dX lo (its rows alone); a4 and a5 after them
+constexpr uint32_t cF = 64;     // [f; F'] of E hi and lo, of E mid, of dX mid and lo (their rows alone); then a4 and a5
 constexpr uint32_t cA = 256;    // a1, a2
-constexpr uint32_t cA3 = 384;   // a3 of E hi, of E lo
+constexpr uint32_t cA3 = 384;   // a3 of E hi and lo, of E mid
 
 struct Bars {
   uint64_t qk_full, qk_empty, ox_full, ox_empty, ex_full, ex_empty;
-  uint64_t a_full, a_empty, b_full, b_empty, c_full, c_empty;  // S0 hi, dS1 hi, the lo slot
+  uint64_t s_full[kRing], s_empty[kRing];  // S0 and dS1, 16 value channels each
   uint64_t g_full[2], g_empty[2];
-  uint64_t f, a, a3, a45;      // MMA groups done
+  uint64_t f, a, a45;          // MMA groups done
   uint64_t nm, free;           // N, M written; all accumulators read
   uint64_t sums, fin;          // the epilogues' sums written; dg, dbeta done with them
   uint64_t epi_sync, aux_sync; // meetings of the epilogue warps, of warps 8-11 (bounded, unlike a barrier instruction)
@@ -66,21 +70,38 @@ struct Small {
 // Offsets from the 1024-byte aligned base, by the padded channel count.
 template <int K>
 struct Layout {
-  int ox, ex, sa, sb, sc, nm, out, small;
+  static constexpr int kPiece = 16 * K * 2;     // 16 state rows of one piece: a 2 KB tile per 64 columns
+  static constexpr int kStep = 6 * kPiece;      // S0 hi, mid, lo, dS1 hi, mid, lo
+  int ox, ex, ring, nm, out, small;
   __host__ __device__ explicit Layout(int VP) {
-    const int img = VP * 128, st = VP * K * 2;
     ox = (K / 64) * kReg;                       // after [Q; K]
-    ex = ox + (VP / 64) * kReg;                 // E hi, E lo, dX lo
-    sa = ex + 3 * img;
-    sb = sa + st;
-    sc = sb + st;
-    const int end = sc + st;
-    nm = VP == 128 ? ex + 2 * img : end;        // N, M: over dX lo once a1, a2 and F' have read it
-    out = VP == 128 ? end : end + 2 * kTile;    // N lo; 32 rows of dq or dk on their way out
+    ex = ox + (VP / 64) * kReg;                 // E hi, mid, lo, dX mid, lo
+    ring = ex + 5 * VP * 128;
+    nm = ring + kRing * kStep;                  // N, M
+    out = nm + 2 * kTile;                       // N lo; 32 rows of dq or dk on their way out
     small = out + kTile;                        // (32 x dstate bf16 fit it)
   }
   __host__ __device__ int bytes() const { return small + static_cast<int>(sizeof(Small)); }
 };
+
+// Columns 8 chunk .. 8 chunk + 7 of a row of an fp32 image.
+__device__ __forceinline__ void load_row8(const float* img, int VP, int row, int chunk, float2 (&v)[4]) {
+  const float4 a = __ldcs(reinterpret_cast<const float4*>(img + image_at(VP, row, 2 * chunk)));
+  const float4 b = __ldcs(reinterpret_cast<const float4*>(img + image_at(VP, row, 2 * chunk + 1)));
+  v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+}
+// Their three pieces as 16-byte chunks at `to`, `stride` bytes apart (the hi piece only where `hi` is set).
+__device__ __forceinline__ void stage_row8(unsigned char* to, int stride, bool hi, const float2 (&v)[4]) {
+  uint32_t h[4], m[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split3(v[i], h[i], m[i], l[i]);
+  if (hi) {
+    *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+    to += stride;
+  }
+  *reinterpret_cast<uint4*>(to) = make_uint4(m[0], m[1], m[2], m[3]);
+  *reinterpret_cast<uint4*>(to + stride) = make_uint4(l[0], l[1], l[2], l[3]);
+}
 
 // Column sums over the warp's 32 lanes: lane l gets column l.
 __device__ __forceinline__ float column_sums(float (&x)[32], int lane) {
@@ -113,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap mdv, const Params p,
                     const TcBuffers w, uint32_t* status) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  const int VP = pad_channels(p.V), img = VP * 128, simg = VP * K * 2;
+  const int VP = pad_channels(p.V), img = VP * 128, steps = VP / 16;
   const Layout<K> lay(VP);
   Small& sm = *reinterpret_cast<Small*>(smem + lay.small);
   Bars& bar = sm.bar;
@@ -123,14 +144,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile uint32_t* fail = &bar.fail;
 
   if (tid == 0) {
-    uint64_t* one[] = {&bar.qk_full, &bar.ox_full, &bar.ox_empty, &bar.ex_full, &bar.ex_empty, &bar.a_full, &bar.b_full,
-                       &bar.c_full, &bar.g_full[0], &bar.g_full[1], &bar.f, &bar.a, &bar.a3, &bar.a45, &bar.fin,
-                       &bar.drain};
+    uint64_t* one[] = {&bar.qk_full, &bar.ox_full, &bar.ox_empty, &bar.ex_empty, &bar.s_empty[0], &bar.s_empty[1],
+                       &bar.g_full[0], &bar.g_full[1], &bar.f, &bar.a, &bar.a45, &bar.fin, &bar.drain};
     for (uint64_t* b : one) mbar_init(b, 1);
     mbar_init(&bar.qk_empty, 1 + kEpi);
-    mbar_init(&bar.a_empty, 1 + kAux);
-    mbar_init(&bar.b_empty, 1 + kAux);
-    mbar_init(&bar.c_empty, 1 + kAux);
+    mbar_init(&bar.ex_full, kAux);
+    for (int i = 0; i < kRing; ++i) mbar_init(&bar.s_full[i], kAux);
     for (int i = 0; i < 2; ++i) mbar_init(&bar.g_empty[i], kEpi + 1);
     mbar_init(&bar.nm, kEpi);
     mbar_init(&bar.free, kEpi);
@@ -181,6 +200,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
           const long long ch = static_cast<long long>(slot) * p.H + h;
           const uint32_t last = (hc - 1) & 1;
+          bulk_prefetch_l2(w.E + ch * token_image(p.V), VP * kC * 4);  // warps 8-11 read these next
+          bulk_prefetch_l2(w.dX + ch * token_image(p.V), VP * kC * 4);
+          bulk_prefetch_l2(w.S + ch * state_image(p.V, K), VP * K * 4);
+          bulk_prefetch_l2(w.dS + ch * state_image(p.V, K), VP * K * 4);
           if (hc > 1 && !(ok = wait1(&bar.g_empty[hc & 1], (hc / 2 - 1) & 1))) break;
           mbar_arrive_expect_tx(&bar.g_full[hc & 1], kGateFloats * 4);
           bulk_g2s(sm.gate[hc & 1], w.gates + ch * kGateFloats, kGateFloats * 4, &bar.g_full[hc & 1]);
@@ -190,22 +213,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d(smem + lay.ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
             tma_load_4d(smem + lay.ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
           }
-          if (hc > 0 && !(ok = wait1(&bar.ex_empty, last))) break;
-          mbar_arrive_expect_tx(&bar.ex_full, 3 * img);
-          bulk_g2s(smem + lay.ex, w.E + ch * 2 * img, 2 * img, &bar.ex_full);
-          bulk_g2s(smem + lay.ex + 2 * img, w.dX + ch * img, img, &bar.ex_full);
-          if (hc > 0 && !(ok = wait1(&bar.a_empty, last))) break;
-          mbar_arrive_expect_tx(&bar.a_full, simg);
-          bulk_g2s(smem + lay.sa, w.S + ch * 2 * simg, simg, &bar.a_full);
-          if (hc > 0 && !(ok = wait1(&bar.c_empty, 1))) break;  // two phases a head: the last one's second
-          mbar_arrive_expect_tx(&bar.c_full, simg);
-          bulk_g2s(smem + lay.sc, w.S + ch * 2 * simg + simg, simg, &bar.c_full);
-          if (hc > 0 && !(ok = wait1(&bar.b_empty, last))) break;
-          mbar_arrive_expect_tx(&bar.b_full, simg);
-          bulk_g2s(smem + lay.sb, w.dS + ch * 2 * simg, simg, &bar.b_full);
-          if (!(ok = wait1(&bar.c_empty, 0))) break;
-          mbar_arrive_expect_tx(&bar.c_full, simg);
-          bulk_g2s(smem + lay.sc, w.dS + ch * 2 * simg + simg, simg, &bar.c_full);
         }
       }
       if (!ok) {  // failed: what was begun lands before the block ends (each barrier's last phase, or an earlier one)
@@ -216,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMma) {  // ---- MMAs
       constexpr uint32_t idKQ = tc::idesc_bf16(128, 64, false, false);
       constexpr uint32_t idF = tc::idesc_bf16(128, 128, false, true);
+      constexpr uint32_t idF64 = tc::idesc_bf16(128, 64, false, true);
       constexpr uint32_t idA = tc::idesc_bf16(128, 128, true, false);
       constexpr uint32_t idMM128 = tc::idesc_bf16(128, 128, true, true);
       constexpr uint32_t idMM = tc::idesc_bf16(128, 64, true, true);
@@ -225,23 +233,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto jstep = [](int s) { return static_cast<uint64_t>((s * 32) >> 4); };
       const uint32_t sb = smem_u32(smem);
       // state columns as lanes: two 64-column regions (dstate 64: the same one twice, the upper lanes are not read)
-      const uint32_t sreg = K == 128 ? static_cast<uint32_t>(img) : 0u, qreg = K == 128 ? kReg : 0u;
+      constexpr uint32_t sreg = K == 128 ? 2048u : 0u, qreg = K == 128 ? kReg : 0u;
       const uint64_t dQK = tc::smem_desc_sw128(sb, 16, 1024), dK = tc::smem_desc_sw128(sb + kTile, 16, 1024);
       const uint64_t dQn = tc::smem_desc_sw128(sb, qreg, 1024), dKn = tc::smem_desc_sw128(sb + kTile, qreg, 1024);
       const uint64_t dOX = tc::smem_desc_sw128(sb + lay.ox, 16, 1024);
-      const uint64_t dE = tc::smem_desc_sw128(sb + lay.ex, img, 1024);         // [E hi | E lo]
-      const uint64_t dEX = tc::smem_desc_sw128(sb + lay.ex, 2 * img, 1024);    // [E hi | dX lo]
-      const uint64_t dXl = tc::smem_desc_sw128(sb + lay.ex + 2 * img, img, 1024);
-      const uint64_t dSA = tc::smem_desc_sw128(sb + lay.sa, sreg, 1024), dSB = tc::smem_desc_sw128(sb + lay.sb, sreg, 1024);
-      const uint64_t dSC = tc::smem_desc_sw128(sb + lay.sc, sreg, 1024);
+      const uint64_t dE = tc::smem_desc_sw128(sb + lay.ex, img, 1024);            // [E hi | E mid]
+      const uint64_t dEm = tc::smem_desc_sw128(sb + lay.ex + img, img, 1024);     // E mid
+      const uint64_t dEl = tc::smem_desc_sw128(sb + lay.ex + 2 * img, img, 1024); // E lo
+      const uint64_t dEXm = tc::smem_desc_sw128(sb + lay.ex, 3 * img, 1024);      // [E hi | dX mid]
+      const uint64_t dEXl = tc::smem_desc_sw128(sb + lay.ex, 4 * img, 1024);      // [E hi | dX lo]
+      const uint64_t dXm = tc::smem_desc_sw128(sb + lay.ex + 3 * img, img, 1024);
+      const uint64_t dXl = tc::smem_desc_sw128(sb + lay.ex + 4 * img, img, 1024);
       const uint64_t dN = tc::smem_desc_sw128(sb + lay.nm, 16, 1024), dM = tc::smem_desc_sw128(sb + lay.nm + kTile, 16, 1024);
       const uint64_t dNl = tc::smem_desc_sw128(sb + lay.out, 16, 1024);
-      const int vs = VP / 16;
-      int n, tok, task = 0, hc = 0;
+      int n, tok, task = 0, hc = 0, rc = 0;
       Seq q;
       bool ok = true;
       for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
-        const int slot = t / p.G, gr = t - slot * p.G;
+        const int slot = t / p.G;
         if (!chunk_at(p, slot, &n, &q, &tok)) continue;
         const int have = q.len - tok;
         const bool cut = have < kC && p.cu != nullptr;  // rows of the next sequence in the tiles
@@ -272,43 +281,44 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int s = 0; s < K / 16; ++s) tc::mma_bf16(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
             }
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cF, dOX + kstep(s), dE + nstep(s), idF, s > 0);
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cF + 128, dEX + nstep(s), dE + nstep(s), idMM, s > 0);
+            for (int s = 0; s < steps; ++s) {
+              tc::mma_bf16(tb + cF, dOX + kstep(s), dE + nstep(s), idF, s > 0);
+              tc::mma_bf16(tb + cF, dOX + kstep(s), dEl + nstep(s), idF64, true);
+              tc::mma_bf16(tb + cF + 128, dEXm + nstep(s), dE + nstep(s), idMM, s > 0);
+              tc::mma_bf16(tb + cF + 128, dEXm + nstep(s), dEm + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cF + 128, dEXl + nstep(s), dE + nstep(s), idMM, true);
+            }
             tc::mma_commit(&bar.f);
           }
           __syncwarp();
-          ok = wait(&bar.a_full, ph);
-          if (!ok) break;
-          if (elect_one()) {
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA, dSA + nstep(s), dOX + kstep(s), idA, s > 0);
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA + 64, dSA + nstep(s), dXl + nstep(s), idMM, true);
-            tc::mma_commit(&bar.a_empty);
+          for (int s = 0; s < steps; ++s, ++rc) {
+            const int st = rc % kRing;
+            ok = wait(&bar.s_full[st], (rc / kRing) & 1);
+            if (!ok) break;
+            const uint32_t at = sb + lay.ring + st * Layout<K>::kStep;
+            constexpr uint64_t pc = Layout<K>::kPiece >> 4;
+            const uint64_t dS = tc::smem_desc_sw128(at, sreg, 1024), dD = tc::smem_desc_sw128(at + 3 * Layout<K>::kPiece, sreg, 1024);
+            if (elect_one()) {
+              tc::mma_bf16(tb + cA, dS, dOX + kstep(s), idA, s > 0);
+              tc::mma_bf16(tb + cA, dS + pc, dOX + kstep(s), idA, true);
+              tc::mma_bf16(tb + cA, dS + 2 * pc, dOX + kstep(s), idA, true);
+              tc::mma_bf16(tb + cA + 64, dS, dXm + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cA + 64, dS + pc, dXm + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cA + 64, dS, dXl + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cA3, dD, dE + nstep(s), idMM128, s > 0);
+              tc::mma_bf16(tb + cA3, dD + pc, dE + nstep(s), idMM128, true);
+              tc::mma_bf16(tb + cA3, dD, dEl + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cA3, dD + 2 * pc, dE + nstep(s), idMM, true);
+              tc::mma_commit(&bar.s_empty[st]);
+              if (s == steps - 1) {
+                tc::mma_commit(&bar.a);
+                tc::mma_commit(&bar.ox_empty);
+                tc::mma_commit(&bar.ex_empty);
+              }
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          ok = wait(&bar.c_full, 0);
           if (!ok) break;
-          if (elect_one()) {
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA, dSC + nstep(s), dOX + kstep(s), idA, true);
-            tc::mma_commit(&bar.a);
-            tc::mma_commit(&bar.c_empty);
-            tc::mma_commit(&bar.ox_empty);
-          }
-          __syncwarp();
-          ok = wait(&bar.b_full, ph);
-          if (!ok) break;
-          if (elect_one()) {
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA3, dSB + nstep(s), dE + nstep(s), idMM128, s > 0);
-            tc::mma_commit(&bar.b_empty);
-          }
-          __syncwarp();
-          ok = wait(&bar.c_full, 1);
-          if (!ok) break;
-          if (elect_one()) {
-            for (int s = 0; s < vs; ++s) tc::mma_bf16(tb + cA3, dSC + nstep(s), dE + nstep(s), idMM, true);
-            tc::mma_commit(&bar.a3);
-            tc::mma_commit(&bar.c_empty);
-          }
-          __syncwarp();
           ok = wait(&bar.nm, ph);
           if (!ok) break;
           tc::fence_after_sync();
@@ -324,7 +334,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
             tc::mma_commit(&bar.a45);
-            tc::mma_commit(&bar.ex_empty);
             if (h == hpg - 1) tc::mma_commit(&bar.qk_empty);
           }
           __syncwarp();
@@ -336,25 +345,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp >= kEpi) {  // ---- <dS1, S0>, dg, dbeta
+  } else if (warp >= kEpi) {  // ---- staging, <dS1, S0>, dg, dbeta
     set_regs_down<kRegAux>();
     const int at = tid - kEpi * 32;
     int n, tok, hc = 0;
     Seq q;
     bool ok = true;
-    auto dot8 = [](uint4 a, uint4 b, float2 acc) {
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc = f2_fma(cvt_pair<__nv_bfloat16>(x[i]), cvt_pair<__nv_bfloat16>(y[i]), acc);
-      return acc;
-    };
-    auto dot = [&](int x, int y, float2 acc) {  // of two state images (the same element in the same place)
-#pragma unroll 4
-      for (int i = at * 16; i < simg; i += kAux * 32 * 16)
-        acc = dot8(*reinterpret_cast<const uint4*>(smem + x + i), *reinterpret_cast<const uint4*>(smem + y + i), acc);
-      return acc;
-    };
-    auto release = [&](uint64_t* b) {
+    int rc = 0;
+    auto publish = [&](uint64_t* b) {
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
@@ -363,18 +362,55 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!chunk_at(p, slot, &n, &q, &tok)) continue;
       for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
         const uint32_t ph = hc & 1;
-        ok = wait(&bar.a_full, ph) && wait(&bar.c_full, 0) && wait(&bar.b_full, ph);
+        const long long ch = static_cast<long long>(slot) * p.H + h;
+        const float *gE = w.E + ch * token_image(p.V), *gX = w.dX + ch * token_image(p.V);
+        const float *gS = w.S + ch * state_image(p.V, K), *gD = w.dS + ch * state_image(p.V, K);
+        // E and dX: 8 chunks of 8 tokens per row
+        ok = hc == 0 || wait(&bar.ex_empty, (hc - 1) & 1);
         if (!ok) break;
-        float2 acc = dot(lay.sa, lay.sb, make_float2(0, 0));
-        float2 low = dot(lay.sc, lay.sb, make_float2(0, 0));  // S0 lo dS1 hi
-        release(&bar.c_empty);
-        release(&bar.b_empty);
-        ok = wait(&bar.c_full, 1);
+#pragma unroll 2
+        for (int i = at; i < VP * 8; i += kAux * 32) {
+          const int row = i & (VP - 1), c = VP == 128 ? i >> 7 : i >> 6;
+          float2 e[4], x[4];
+          load_row8(gE, VP, row, c, e);
+          load_row8(gX, VP, row, c, x);
+          unsigned char* to = smem + lay.ex + tc::chunk_off(row, c);
+          stage_row8(to, img, true, e);
+          stage_row8(to + 3 * img, img, false, x);  // dX hi is dv
+        }
+        publish(&bar.ex_full);
+        // S0 and dS1, 16 rows a step: K / 8 chunks per row
+        float2 acc = make_float2(0, 0);
+        constexpr int kItems = 16 * (K / 8) / (kAux * 32);  // chunks of a thread and step: 1 (dstate 64) or 2
+        float2 s0[kItems][4], d1[kItems][4];
+        auto fetch = [&](int s) {
+#pragma unroll
+          for (int k = 0; k < kItems; ++k) {
+            const int i = at + k * kAux * 32;
+            load_row8(gS, VP, 16 * s + (i & 15), i >> 4, s0[k]);
+            load_row8(gD, VP, 16 * s + (i & 15), i >> 4, d1[k]);
+          }
+        };
+        fetch(0);
+        for (int s = 0; s < steps; ++s, ++rc) {
+          const int st = rc % kRing;
+          ok = rc < kRing || wait(&bar.s_empty[st], (rc / kRing - 1) & 1);
+          if (!ok) break;
+          unsigned char* base = smem + lay.ring + st * Layout<K>::kStep;
+#pragma unroll
+          for (int k = 0; k < kItems; ++k) {
+            const int i = at + k * kAux * 32, row = i & 15, c = i >> 4;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) acc = f2_fma(s0[k][m], d1[k][m], acc);
+            unsigned char* to = base + (c >> 3) * 2048 + tc::chunk_off(row, c & 7);
+            stage_row8(to, Layout<K>::kPiece, true, s0[k]);
+            stage_row8(to + 3 * Layout<K>::kPiece, Layout<K>::kPiece, true, d1[k]);
+          }
+          publish(&bar.s_full[st]);
+          if (s + 1 < steps) fetch(s + 1);
+        }
         if (!ok) break;
-        low = dot(lay.sa, lay.sc, low);
-        release(&bar.c_empty);
-        release(&bar.a_empty);
-        float d = (acc.x + acc.y) + (low.x + low.y);
+        float d = acc.x + acc.y;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
         if (lane == 0) sm.dot[warp - kEpi] = d;
@@ -475,7 +511,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) x[k] = c0 + k <= lim ? sc * __expf(bi - gate[kGateB + c0 + k]) * x[k] : 0.f;
           ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
-          ok = ok && wait(&bar.a, ph);                   // dX lo has been read where N and M go
           if (!ok) break;
           unsigned char* tile = smem + lay.nm + (second ? kTile : 0);
 #pragma unroll
@@ -514,7 +549,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           sm.y[quarter][c0 + lane] = y;
           sm.R[quarter][c0 + lane] = Rs;
         }
-        // state columns as lanes: a1, a2, a3 (bar.a has completed)
+        // state columns as lanes: a1, a2, a3
+        ok = wait(&bar.a, ph);
+        if (!ok) break;
         tc::fence_after_sync();
         {
           const unsigned char* tq = smem + (K == 128 ? (row >> 6) * kReg : 0);
@@ -543,9 +580,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           sm.r[quarter][c0 + lane] = column_sums(s, lane);
-          ok = wait(&bar.a3, ph);
-          if (!ok) break;
-          tc::fence_after_sync();
           {
             float a[32], b[32];
             tmem_ld32(tb + tl + cA3 + c0, a);

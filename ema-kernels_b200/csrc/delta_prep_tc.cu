@@ -2,7 +2,7 @@
 //
 //   gates:  b_i (running sum of g), exp(b_i), exp(b_end - b_i), beta_i, exp(b_end)
 //   P_ij = scale exp(b_i - b_j) (q_i . k_j)  for j <= i
-//   T = (I + A)^-1,  A_ij = exp(b_i - b_j) (k_i . k_j) beta_j  for j < i
+//   T - I,  T = (I + A)^-1,  A_ij = exp(b_i - b_j) (k_i . k_j) beta_j  for j < i
 //
 // One block per (chunk, group, up to kHeads of its heads).  K K^t and Q K^t are one M = 128 MMA chain,
 // [K; Q] K^t, read once into registers (a thread owns one of the 128 rows) and scaled per head.  The
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_tc_kernel(const __grid_const
           v[c] = f.x, v[c + 1] = f.y, v[c + 2] = f.z, v[c + 3] = f.w;
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = c0 + 16 * g + k <= r ? v[k] : 0.f;
+        for (int k = 0; k < 16; ++k) v[k] = c0 + 16 * g + k < r ? v[k] : 0.f;
         store_row16(to, to + kTile, r, c0 + 16 * g, v);
       }
     }

@@ -2,16 +2,15 @@
 // operand images, and 32-bit precision out of bf16 products.
 //
 // Precision.  States, gate gradients and every other fp32 output have to be good to fp32's own order, so a product's
-// operand that is not bf16 by nature (T, X, U, S, dX, dS) enters as a pair of bf16: hi = bf16(x), lo = bf16(x - hi),
-// x = hi + lo to 2^-17.  A bf16 tensor times a pair is two MMAs, a pair times a pair three (lo lo is dropped at
-// 2^-18).  Only what ends in a bf16 output alone (o's two terms, dq and dk) uses the hi parts.
+// operand that is not bf16 by nature enters as two bf16 pieces, hi = bf16(x), lo = bf16(x - hi), x = hi + lo to
+// 2^-16, or as three (2^-24) where the sums that follow cancel: what the gate gradients are summed from (E, dX, S0 and
+// dS1 in the gradient kernel).  A bf16 tensor times a pair is two MMAs, a pair times a pair three (lo lo is dropped), three
+// pieces times three six.  T enters without its unit diagonal, which is added in fp32 from the operand itself.
 //
-// Images.  What one kernel leaves for the next as an MMA operand lies in global memory as the 128-byte swizzled
-// tile that shared memory wants (rows of 64 bf16, 16-byte chunk c of row r at c ^ (r % 8)), so that a plain
-// bulk copy stages it and the writing thread stores whole 16-byte chunks of its own row:
-//   T, P   64 x 64, row = token i, column = token j: hi, lo (8 KB each)
-//   E, dX  row = value channel, column = token: hi, lo
-//   S, dS  row = value channel, one region per 64 state columns: hi regions, lo regions
+// Images.  T and P lie in global memory as the 128-byte swizzled bf16 tiles that shared memory wants (rows of 64 bf16,
+// 16-byte chunk c of row r at c ^ (r % 8)), so that a plain bulk copy stages them: 64 x 64, row = token i, column =
+// token j, hi then lo (8 KB each).  S, dS, E and dX are fp32, for a thread that owns the row of a value channel:
+// four columns after four columns, each with all the rows, so that a warp stores and loads 512 bytes in a piece.
 #pragma once
 
 #include "delta_common.cuh"
@@ -28,22 +27,32 @@ constexpr int kGateE = 0, kGateW = 64, kGateBeta = 128, kGateB = 192, kGateEnd =
 
 struct TcBuffers {
   float* gates;      // kGateFloats per (slot, head)
-  char* T;           // hi, lo
+  char* T;           // T - I: hi, lo
   char* P;           // hi, lo
-  char* S;           // state entering the chunk: hi, lo (null: not kept)
-  char* E;           // hi, lo (null: not kept)
-  char* dS;          // gradient of the state at the chunk's end: hi, lo
-  char* dX;          // lo
+  float* S;          // state entering the chunk (null: not kept)
+  float* E;          // (null: not kept)
+  float* dS;         // gradient of the state at the chunk's end
+  float* dX;
 };
 
 __host__ __device__ inline int pad_channels(int V) { return V <= 64 ? 64 : 128; }
-__host__ __device__ inline size_t state_image(int V, int K) { return static_cast<size_t>(pad_channels(V)) * K * 2; }
-__host__ __device__ inline size_t token_image(int V) { return static_cast<size_t>(pad_channels(V)) * 128; }
+// Floats of an image, and the place of columns 4 piece .. 4 piece + 3 of a row in it.
+__host__ __device__ inline size_t state_image(int V, int K) { return static_cast<size_t>(pad_channels(V)) * K; }
+__host__ __device__ inline size_t token_image(int V) { return static_cast<size_t>(pad_channels(V)) * kC; }
+__device__ __forceinline__ int image_at(int VP, int row, int piece) { return (piece * VP + row) * 4; }
 
 // bf16 pair (x, y) -> packed hi and packed lo.
 __device__ __forceinline__ void split2(float2 v, uint32_t& hi, uint32_t& lo) {
   hi = pack_pair<__nv_bfloat16>(v);
   lo = pack_pair<__nv_bfloat16>(f2_fma(cvt_pair<__nv_bfloat16>(hi), make_float2(-1.f, -1.f), v));
+}
+
+// Three pieces.
+__device__ __forceinline__ void split3(float2 v, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = pack_pair<__nv_bfloat16>(v);
+  const float2 r = f2_fma(cvt_pair<__nv_bfloat16>(hi), make_float2(-1.f, -1.f), v);
+  mid = pack_pair<__nv_bfloat16>(r);
+  lo = pack_pair<__nv_bfloat16>(f2_fma(cvt_pair<__nv_bfloat16>(mid), make_float2(-1.f, -1.f), r));
 }
 
 // D[tmem] (+)= A[tmem] B^T for one K = 16 step: A's 16 columns are 8 packed 32-bit tensor-memory columns.
