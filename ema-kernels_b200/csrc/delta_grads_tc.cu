@@ -11,16 +11,17 @@
 // and what the gates need, by transposed butterflies over the lanes of fp32 values:
 //   dbeta_j = sum of y over its column + w_j k_j . a3_j
 //   dg_t = sum over rows of (prefix of beta y up to t) + sum_{i >= t} r_i + sum_{j < t} c_j + exp(b_end) <dS1, S0>
-// dg and dbeta are fp32 results, and sums that cancel: S0, dS1, E and dX enter as three bf16 pieces each, all products of
-// them down to 2^-24.  N is a pair where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are
+// dg and dbeta are fp32 results, and sums that cancel: S0, dS1 and E enter as three bf16 pieces each, dX as two (dv and the
+// rest), with all products of them down to 2^-24.  N is a pair where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are
 // single bf16.
 //
 // One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  S0, dS1, E
 // and dX come as fp32 images; warps 8-11 take them through registers, sum <dS1, S0> on the way and stage the pieces, S0 and
 // dS1 in steps of 16 value channels (one MMA step) through a ring of two.  Bound: the images' bytes (S0 and dS1 are 2 x 64
 // KB a chunk and head at 128 x 128), and near it the tensor pipe (about 7500 cycles a head) and the epilogues.  Roles: warps
-// 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 staging and the gates' results, warp 12 the MMAs, warp
-// 13 the loads of Q, K, dO and dv.
+// 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 staging, warp 12 the MMAs, warp 13 the loads of Q, K, dO
+// and dv, warp 14 dg and dbeta from the epilogues' sums.  The long loops are kept rolled where they can be: at twice the
+// code the block ran at a third of the speed, waiting for instructions.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -34,16 +35,16 @@ namespace delta {
 namespace {
 
 constexpr int kEpi = 8, kAux = 4;
-constexpr int kMma = 12, kLoad = 13;  // (14 and 15 only fill their warpgroup)
+constexpr int kMma = 12, kLoad = 13, kGates = 14;  // (15 only fills its warpgroup)
 constexpr int kThreads = 16 * 32;
-constexpr int kRegEpi = 168, kRegAux = 112, kRegCtl = 64;
-static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128, "register split");
+constexpr int kRegEpi = 160, kRegAux = 136, kRegCtl = 56;
+static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128 && kRegAux >= 128 && kRegCtl <= 128, "register split");
 constexpr int kRing = 2;
 constexpr int kReg = 128 * 128;  // two 64-row tiles of 64 columns, one over the other
 
 // tensor-memory columns
 constexpr uint32_t cKQ = 0;     // [qk; kk]
-constexpr uint32_t cF = 64;     // [f; F'] of E hi and lo, of E mid, of dX mid and lo (their rows alone); then a4 and a5
+constexpr uint32_t cF = 64;     // [f; F'] of E hi and lo, of E mid, of dX lo (its rows alone); then a4 and a5
 constexpr uint32_t cA = 256;    // a1, a2
 constexpr uint32_t cA3 = 384;   // a3 of E hi and lo, of E mid
 
@@ -53,8 +54,8 @@ struct Bars {
   uint64_t g_full[2], g_empty[2];
   uint64_t f, a, a45;          // MMA groups done
   uint64_t nm, free;           // N, M written; all accumulators read
-  uint64_t sums, fin;          // the epilogues' sums written; dg, dbeta done with them
-  uint64_t epi_sync, aux_sync; // meetings of the epilogue warps, of warps 8-11 (bounded, unlike a barrier instruction)
+  uint64_t sums, fin;          // the epilogues' sums and <dS1, S0> written; dg, dbeta done with them
+  uint64_t epi_sync;           // meeting of the epilogue warps (bounded, unlike a barrier instruction)
   uint64_t drain;
   uint32_t taddr, fail;
 };
@@ -75,8 +76,8 @@ struct Layout {
   int ox, ex, ring, nm, out, small;
   __host__ __device__ explicit Layout(int VP) {
     ox = (K / 64) * kReg;                       // after [Q; K]
-    ex = ox + (VP / 64) * kReg;                 // E hi, mid, lo, dX mid, lo
-    ring = ex + 5 * VP * 128;
+    ex = ox + (VP / 64) * kReg;                 // E hi, mid, lo, dX lo
+    ring = ex + 4 * VP * 128;
     nm = ring + kRing * kStep;                  // N, M
     out = nm + 2 * kTile;                       // N lo; 32 rows of dq or dk on their way out
     small = out + kTile;                        // (32 x dstate bf16 fit it)
@@ -90,17 +91,21 @@ __device__ __forceinline__ void load_row8(const float* img, int VP, int row, int
   const float4 b = __ldcs(reinterpret_cast<const float4*>(img + image_at(VP, row, 2 * chunk + 1)));
   v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
 }
-// Their three pieces as 16-byte chunks at `to`, `stride` bytes apart (the hi piece only where `hi` is set).
-__device__ __forceinline__ void stage_row8(unsigned char* to, int stride, bool hi, const float2 (&v)[4]) {
+// Their three pieces as 16-byte chunks at `to`, `stride` bytes apart.
+__device__ __forceinline__ void stage_row8(unsigned char* to, int stride, const float2 (&v)[4]) {
   uint32_t h[4], m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) split3(v[i], h[i], m[i], l[i]);
-  if (hi) {
-    *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-    to += stride;
-  }
-  *reinterpret_cast<uint4*>(to) = make_uint4(m[0], m[1], m[2], m[3]);
-  *reinterpret_cast<uint4*>(to + stride) = make_uint4(l[0], l[1], l[2], l[3]);
+  *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(to + stride) = make_uint4(m[0], m[1], m[2], m[3]);
+  *reinterpret_cast<uint4*>(to + 2 * stride) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// The second piece alone.
+__device__ __forceinline__ void stage_lo8(unsigned char* to, const float2 (&v)[4]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split2(v[i], h[i], l[i]);
+  *reinterpret_cast<uint4*>(to) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 // Column sums over the warp's 32 lanes: lane l gets column l.
@@ -153,9 +158,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) mbar_init(&bar.g_empty[i], kEpi + 1);
     mbar_init(&bar.nm, kEpi);
     mbar_init(&bar.free, kEpi);
-    mbar_init(&bar.sums, kEpi);
+    mbar_init(&bar.sums, kEpi + kAux);
     mbar_init(&bar.epi_sync, kEpi);
-    mbar_init(&bar.aux_sync, kAux);
     bar.fail = 0;
     fence_mbar_init();
   }
@@ -240,10 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dE = tc::smem_desc_sw128(sb + lay.ex, img, 1024);            // [E hi | E mid]
       const uint64_t dEm = tc::smem_desc_sw128(sb + lay.ex + img, img, 1024);     // E mid
       const uint64_t dEl = tc::smem_desc_sw128(sb + lay.ex + 2 * img, img, 1024); // E lo
-      const uint64_t dEXm = tc::smem_desc_sw128(sb + lay.ex, 3 * img, 1024);      // [E hi | dX mid]
-      const uint64_t dEXl = tc::smem_desc_sw128(sb + lay.ex, 4 * img, 1024);      // [E hi | dX lo]
-      const uint64_t dXm = tc::smem_desc_sw128(sb + lay.ex + 3 * img, img, 1024);
-      const uint64_t dXl = tc::smem_desc_sw128(sb + lay.ex + 4 * img, img, 1024);
+      const uint64_t dEX = tc::smem_desc_sw128(sb + lay.ex, 3 * img, 1024);       // [E hi | dX lo]
+      const uint64_t dXl = tc::smem_desc_sw128(sb + lay.ex + 3 * img, img, 1024);
       const uint64_t dN = tc::smem_desc_sw128(sb + lay.nm, 16, 1024), dM = tc::smem_desc_sw128(sb + lay.nm + kTile, 16, 1024);
       const uint64_t dNl = tc::smem_desc_sw128(sb + lay.out, 16, 1024);
       int n, tok, task = 0, hc = 0, rc = 0;
@@ -278,19 +280,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::fence_after_sync();
           if (elect_one()) {
             if (h == 0) {
-#pragma unroll
+#pragma unroll 1
               for (int s = 0; s < K / 16; ++s) tc::mma_bf16(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
             }
+#pragma unroll 1
             for (int s = 0; s < steps; ++s) {
               tc::mma_bf16(tb + cF, dOX + kstep(s), dE + nstep(s), idF, s > 0);
               tc::mma_bf16(tb + cF, dOX + kstep(s), dEl + nstep(s), idF64, true);
-              tc::mma_bf16(tb + cF + 128, dEXm + nstep(s), dE + nstep(s), idMM, s > 0);
-              tc::mma_bf16(tb + cF + 128, dEXm + nstep(s), dEm + nstep(s), idMM, true);
-              tc::mma_bf16(tb + cF + 128, dEXl + nstep(s), dE + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cF + 128, dEX + nstep(s), dE + nstep(s), idMM, s > 0);
+              tc::mma_bf16(tb + cF + 128, dEX + nstep(s), dEm + nstep(s), idMM, true);
             }
             tc::mma_commit(&bar.f);
           }
           __syncwarp();
+#pragma unroll 1
           for (int s = 0; s < steps; ++s, ++rc) {
             const int st = rc % kRing;
             ok = wait(&bar.s_full[st], (rc / kRing) & 1);
@@ -302,9 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc::mma_bf16(tb + cA, dS, dOX + kstep(s), idA, s > 0);
               tc::mma_bf16(tb + cA, dS + pc, dOX + kstep(s), idA, true);
               tc::mma_bf16(tb + cA, dS + 2 * pc, dOX + kstep(s), idA, true);
-              tc::mma_bf16(tb + cA + 64, dS, dXm + nstep(s), idMM, true);
-              tc::mma_bf16(tb + cA + 64, dS + pc, dXm + nstep(s), idMM, true);
               tc::mma_bf16(tb + cA + 64, dS, dXl + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cA + 64, dS + pc, dXl + nstep(s), idMM, true);
               tc::mma_bf16(tb + cA3, dD, dE + nstep(s), idMM128, s > 0);
               tc::mma_bf16(tb + cA3, dD + pc, dE + nstep(s), idMM128, true);
               tc::mma_bf16(tb + cA3, dD, dEl + nstep(s), idMM, true);
@@ -323,16 +325,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc::fence_after_sync();
           if (elect_one()) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + nstep(s), idMM, true);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) tc::mma_bf16(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
+#pragma unroll 1
+            for (int s = 0; s < 4; ++s) {
+              tc::mma_bf16(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
+              tc::mma_bf16(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
+              tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
+              tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + nstep(s), idMM, true);
+              tc::mma_bf16(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
+            }
             tc::mma_commit(&bar.a45);
             if (h == hpg - 1) tc::mma_commit(&bar.qk_empty);
           }
@@ -345,13 +345,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp >= kEpi) {  // ---- staging, <dS1, S0>, dg, dbeta
-    set_regs_down<kRegAux>();
+    if (warp == kGates) {  // ---- dg, dbeta
+      int n, tok, hc = 0;
+      Seq q;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
+        const int slot = t / p.G, gr = t - slot * p.G;
+        if (!chunk_at(p, slot, &n, &q, &tok)) continue;
+        for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
+          ok = wait(&bar.g_full[hc & 1], (hc / 2) & 1) && wait(&bar.sums, hc & 1);
+          if (!ok) break;
+          const float* gate = sm.gate[hc & 1];
+          const float all = ((sm.dot[0] + sm.dot[1]) + (sm.dot[2] + sm.dot[3])) * gate[kGateEnd];
+          float y[2], r[2], R[2], c[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int j = 2 * lane + k;
+            y[k] = (sm.y[0][j] + sm.y[1][j]) + (sm.y[2][j] + sm.y[3][j]);
+            r[k] = (sm.r[0][j] + sm.r[1][j]) + (sm.r[2][j] + sm.r[3][j]);
+            R[k] = (sm.R[0][j] + sm.R[1][j]) + (sm.R[2][j] + sm.R[3][j]);
+            c[k] = (sm.c[0][j] + sm.c[1][j]) + (sm.c[2][j] + sm.c[3][j]);  // w_j k_j . a3_j
+          }
+          const float b0 = gate[kGateBeta + 2 * lane], b1 = gate[kGateBeta + 2 * lane + 1];
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bar.fin);
+            mbar_arrive(&bar.g_empty[hc & 1]);
+          }
+          float pre = b0 * c[0] + b1 * c[1], suf = r[0] + r[1];  // sums up to and from this lane's tokens
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float a = __shfl_up_sync(0xffffffffu, pre, o), b = __shfl_down_sync(0xffffffffu, suf, o);
+            if (lane >= o) pre += a;
+            if (lane + o < 32) suf += b;
+          }
+          const float before = __shfl_up_sync(0xffffffffu, pre, 1);
+          const float after = __shfl_down_sync(0xffffffffu, suf, 1);
+          const float pre0 = lane > 0 ? before : 0.f, suf1 = r[1] + (lane < 31 ? after : 0.f);
+          const float dg[2] = {R[0] + (suf1 + r[0]) + pre0 + all, R[1] + suf1 + (pre0 + b0 * c[0]) + all};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int j = 2 * lane + k;
+            if (tok + j < q.len) {
+              const long long to = (static_cast<long long>(q.b) * p.L + q.t0 + tok + j) * p.H + h;
+              p.dg[to] = p.g[to] > kMinGate ? dg[k] : 0.f;  // a clamped gate has no gradient
+              p.dbeta[to] = y[k] + c[k];
+            }
+          }
+        }
+      }
+    }
+  } else if (warp >= kEpi) {  // ---- staging, <dS1, S0>
+    set_regs_up<kRegAux>();
     const int at = tid - kEpi * 32;
-    int n, tok, hc = 0;
+    int n, tok, hc = 0, rc = 0;
     Seq q;
     bool ok = true;
-    int rc = 0;
     auto publish = [&](uint64_t* b) {
       fence_proxy_async_smem();
       __syncwarp();
@@ -361,105 +410,79 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int slot = t / p.G, gr = t - slot * p.G;
       if (!chunk_at(p, slot, &n, &q, &tok)) continue;
       for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
-        const uint32_t ph = hc & 1;
         const long long ch = static_cast<long long>(slot) * p.H + h;
         const float *gE = w.E + ch * token_image(p.V), *gX = w.dX + ch * token_image(p.V);
         const float *gS = w.S + ch * state_image(p.V, K), *gD = w.dS + ch * state_image(p.V, K);
-        // E and dX: 8 chunks of 8 tokens per row
-        ok = hc == 0 || wait(&bar.ex_empty, (hc - 1) & 1);
-        if (!ok) break;
-#pragma unroll 2
-        for (int i = at; i < VP * 8; i += kAux * 32) {
-          const int row = i & (VP - 1), c = VP == 128 ? i >> 7 : i >> 6;
-          float2 e[4], x[4];
-          load_row8(gE, VP, row, c, e);
-          load_row8(gX, VP, row, c, x);
-          unsigned char* to = smem + lay.ex + tc::chunk_off(row, c);
-          stage_row8(to, img, true, e);
-          stage_row8(to + 3 * img, img, false, x);  // dX hi is dv
-        }
-        publish(&bar.ex_full);
-        // S0 and dS1, 16 rows a step: K / 8 chunks per row
+        // E and dX: 8 chunks of 8 tokens per row, two of each in flight; the first steps of S0 and dS1 on their way meanwhile
+        float2 e[2][4], x[2][4];
+        const int row = at & (VP - 1), c0 = VP == 128 ? 0 : at >> 6, cs = VP == 128 ? 1 : 2;
+        auto fetch2 = [&](int c) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            load_row8(gE, VP, row, c + k * cs, e[k]);
+            load_row8(gX, VP, row, c + k * cs, x[k]);
+          }
+        };
+        // S0 and dS1, 16 rows a step: K / 8 chunks per row, two steps in flight
         float2 acc = make_float2(0, 0);
         constexpr int kItems = 16 * (K / 8) / (kAux * 32);  // chunks of a thread and step: 1 (dstate 64) or 2
-        float2 s0[kItems][4], d1[kItems][4];
-        auto fetch = [&](int s) {
+        float2 s0[2][kItems][4], d1[2][kItems][4];
+        auto fetch = [&](int s, int into) {
 #pragma unroll
           for (int k = 0; k < kItems; ++k) {
             const int i = at + k * kAux * 32;
-            load_row8(gS, VP, 16 * s + (i & 15), i >> 4, s0[k]);
-            load_row8(gD, VP, 16 * s + (i & 15), i >> 4, d1[k]);
+            load_row8(gS, VP, 16 * s + (i & 15), i >> 4, s0[into][k]);
+            load_row8(gD, VP, 16 * s + (i & 15), i >> 4, d1[into][k]);
           }
         };
-        fetch(0);
-        for (int s = 0; s < steps; ++s, ++rc) {
-          const int st = rc % kRing;
-          ok = rc < kRing || wait(&bar.s_empty[st], (rc / kRing - 1) & 1);
-          if (!ok) break;
-          unsigned char* base = smem + lay.ring + st * Layout<K>::kStep;
+        fetch2(c0);
+        fetch(0, 0);
+        ok = hc == 0 || wait(&bar.ex_empty, (hc - 1) & 1);
+        if (!ok) break;
+#pragma unroll 1
+        for (int c = c0; c < 8; c += 2 * cs) {
 #pragma unroll
-          for (int k = 0; k < kItems; ++k) {
-            const int i = at + k * kAux * 32, row = i & 15, c = i >> 4;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) acc = f2_fma(s0[k][m], d1[k][m], acc);
-            unsigned char* to = base + (c >> 3) * 2048 + tc::chunk_off(row, c & 7);
-            stage_row8(to, Layout<K>::kPiece, true, s0[k]);
-            stage_row8(to + 3 * Layout<K>::kPiece, Layout<K>::kPiece, true, d1[k]);
+          for (int k = 0; k < 2; ++k) {
+            unsigned char* to = smem + lay.ex + tc::chunk_off(row, c + k * cs);
+            stage_row8(to, img, e[k]);
+            stage_lo8(to + 3 * img, x[k]);  // dX hi is dv
           }
-          publish(&bar.s_full[st]);
-          if (s + 1 < steps) fetch(s + 1);
+          if (c + 2 * cs < 8) fetch2(c + 2 * cs);
+        }
+        publish(&bar.ex_full);
+        fetch(1, 1);
+#pragma unroll 1
+        for (int s2 = 0; ok && s2 < steps; s2 += 2) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u, ++rc) {
+            const int st = rc % kRing;
+            ok = ok && (rc < kRing || wait(&bar.s_empty[st], (rc / kRing - 1) & 1));
+            if (!ok) break;
+            unsigned char* base = smem + lay.ring + st * Layout<K>::kStep;
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+              const int i = at + k * kAux * 32, r = i & 15, c = i >> 4;
+#pragma unroll
+              for (int m = 0; m < 4; ++m) acc = f2_fma(s0[u][k][m], d1[u][k][m], acc);
+              unsigned char* to = base + (c >> 3) * 2048 + tc::chunk_off(r, c & 7);
+              stage_row8(to, Layout<K>::kPiece, s0[u][k]);
+              stage_row8(to + 3 * Layout<K>::kPiece, Layout<K>::kPiece, d1[u][k]);
+            }
+            publish(&bar.s_full[st]);
+            if (s2 + 2 < steps) fetch(s2 + 2 + u, u);
+          }
         }
         if (!ok) break;
         float d = acc.x + acc.y;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        if (lane == 0) sm.dot[warp - kEpi] = d;
-        ok = meet(&bar.aux_sync);
-        if (ok && warp == kEpi) {
-          ok = wait(&bar.g_full[hc & 1], (hc / 2) & 1) && wait(&bar.sums, ph);
-          if (ok) {
-            const float* gate = sm.gate[hc & 1];
-            const float all = ((sm.dot[0] + sm.dot[1]) + (sm.dot[2] + sm.dot[3])) * gate[kGateEnd];
-            float y[2], r[2], R[2], c[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int j = 2 * lane + k;
-              y[k] = (sm.y[0][j] + sm.y[1][j]) + (sm.y[2][j] + sm.y[3][j]);
-              r[k] = (sm.r[0][j] + sm.r[1][j]) + (sm.r[2][j] + sm.r[3][j]);
-              R[k] = (sm.R[0][j] + sm.R[1][j]) + (sm.R[2][j] + sm.R[3][j]);
-              c[k] = (sm.c[0][j] + sm.c[1][j]) + (sm.c[2][j] + sm.c[3][j]);  // w_j k_j . a3_j
-            }
-            const float b0 = gate[kGateBeta + 2 * lane], b1 = gate[kGateBeta + 2 * lane + 1];
-            float pre = b0 * c[0] + b1 * c[1], suf = r[0] + r[1];  // sums up to and from this lane's tokens
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const float a = __shfl_up_sync(0xffffffffu, pre, o), b = __shfl_down_sync(0xffffffffu, suf, o);
-              if (lane >= o) pre += a;
-              if (lane + o < 32) suf += b;
-            }
-            const float before = __shfl_up_sync(0xffffffffu, pre, 1);
-            const float after = __shfl_down_sync(0xffffffffu, suf, 1);
-            const float pre0 = lane > 0 ? before : 0.f, suf1 = r[1] + (lane < 31 ? after : 0.f);
-            const float dg[2] = {R[0] + (suf1 + r[0]) + pre0 + all, R[1] + suf1 + (pre0 + b0 * c[0]) + all};
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int j = 2 * lane + k;
-              if (tok + j < q.len) {
-                const long long to = (static_cast<long long>(q.b) * p.L + q.t0 + tok + j) * p.H + h;
-                p.dg[to] = p.g[to] > kMinGate ? dg[k] : 0.f;  // a clamped gate has no gradient
-                p.dbeta[to] = y[k] + c[k];
-              }
-            }
-          }
-          __syncwarp();
-          if (ok && lane == 0) {
-            mbar_arrive(&bar.fin);
-            mbar_arrive(&bar.g_empty[hc & 1]);
-          }
-          __syncwarp();
-        }
-        ok = ok && meet(&bar.aux_sync);  // sm.dot has been read
+        ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
         if (!ok) break;
+        if (lane == 0) {
+          sm.dot[warp - kEpi] = d;
+          mbar_arrive(&bar.sums);
+        }
+        __syncwarp();
       }
     }
   } else {  // ---- epilogues
@@ -498,18 +521,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 32; ++k) x[k] += a[k];
-            if (second) {
-              tmem_ld32(tb + tl + cF + 128 + c0, a);
-              tc::tmem_wait_ld();
+            const float own = second ? 1.f : 0.f;  // (the upper rows of the third part are E E^t)
+            tmem_ld32(tb + tl + cF + 128 + c0, a);
+            tc::tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] += a[k];
-            }
+            for (int k = 0; k < 32; ++k) x[k] = fmaf(own, a[k], x[k]);
           }
           const float bi = gate[kGateB + i];
           const float sc = second ? -1.f : p.scale;
-          const int lim = second ? i - 1 : i;  // last column of the row
+          const int lim = (second ? i - 1 : i) - c0;  // last of these columns in the row
+          const uint32_t wide = __float_as_uint(gate[kGateWide]);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = c0 + k <= lim ? sc * __expf(bi - gate[kGateB + c0 + k]) * x[k] : 0.f;
+          for (int g = 0; g < 2; ++g) {
+            float f[16];
+            if ((wide >> (8 * (2 * hf + g))) & 1u) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) f[k] = sc * __expf(bi - gate[kGateB + c0 + 16 * g + k]);
+            } else {
+              const float rf = sc * __expf(bi - gate[kGateB + c0 + 16 * g]);
+#pragma unroll
+              for (int k = 0; k < 16; k += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(gate + kGateKey + c0 + 16 * g + k);
+                f[k] = rf * k4.x, f[k + 1] = rf * k4.y, f[k + 2] = rf * k4.z, f[k + 3] = rf * k4.w;
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[16 * g + k] = 16 * g + k <= lim ? f[k] * x[16 * g + k] : 0.f;
+          }
           ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
           if (!ok) break;
           unsigned char* tile = smem + lay.nm + (second ? kTile : 0);
@@ -533,10 +571,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           // y, and the prefixes of beta y along the row that reach column t <= i
           float R[32], run = 0.f;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            x[k] *= prod[k];
-            R[k] = run;
-            run = fmaf(gate[kGateBeta + c0 + k], x[k], run);
+          for (int k = 0; k < 32; k += 4) {
+            const float4 b4 = *reinterpret_cast<const float4*>(gate + kGateBeta + c0 + k);
+            const float be[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              x[k + m] *= prod[k + m];
+              R[k + m] = run;
+              run = fmaf(be[m], x[k + m], run);
+            }
           }
           if (hf == 0) sm.base[row] = run;
           const float y = column_sums(x, lane);
@@ -544,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           const float base = hf == 0 ? 0.f : sm.base[row];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) R[k] = c0 + k <= i ? R[k] + base : 0.f;
+          for (int k = 0; k < 32; ++k) R[k] = k <= i - c0 ? R[k] + base : 0.f;
           const float Rs = column_sums(R, lane);
           sm.y[quarter][c0 + lane] = y;
           sm.R[quarter][c0 + lane] = Rs;
@@ -554,30 +597,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc::fence_after_sync();
         {
-          const unsigned char* tq = smem + (K == 128 ? (row >> 6) * kReg : 0);
+          // (dstate 64: lanes 64 and above hold nothing; they read the lower lanes' elements and count for nothing)
+          const unsigned char* tq = smem + (K == 128 ? (row >> 6) * kReg : 0) + c0 * 128;
           const uint32_t col = (row & 63) * 2;
-          auto elem = [&](const unsigned char* tile, int tk) {
-            return klive ? to_f32(*reinterpret_cast<const __nv_bfloat16*>(tile + tk * 128 + (col ^ ((tk & 7) << 4)))) : 0.f;
+          auto elem = [&](const unsigned char* tile, int k) {
+            return to_f32(*reinterpret_cast<const __nv_bfloat16*>(tile + k * 128 + (col ^ ((k & 7) << 4))));
           };
-          float s[32];
+          float s[32], kv[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) kv[k] = elem(tq + kTile, k);
           {
             float a[32];
             tmem_ld32(tb + tl + cA + c0, a);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float v = -p.scale * gate[kGateE + c0 + k] * a[k];
-              dq[k] += v;
-              s[k] = v * elem(tq, c0 + k);
+            for (int k = 0; k < 32; k += 2) {
+              const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + c0 + k);
+              const float v0 = -p.scale * e.x * a[k], v1 = -p.scale * e.y * a[k + 1];
+              dq[k] += v0;
+              dq[k + 1] += v1;
+              s[k] = v0 * elem(tq, k);
+              s[k + 1] = v1 * elem(tq, k + 1);
             }
             tmem_ld32(tb + tl + cA + 64 + c0, a);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float v = gate[kGateE + c0 + k] * a[k];
-              dk[k] += v;
-              s[k] = klive ? fmaf(v, elem(tq + kTile, c0 + k), s[k]) : 0.f;
+            for (int k = 0; k < 32; k += 2) {
+              const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + c0 + k);
+              const float v0 = e.x * a[k], v1 = e.y * a[k + 1];
+              dk[k] += v0;
+              dk[k + 1] += v1;
+              s[k] = fmaf(v0, kv[k], s[k]);
+              s[k + 1] = fmaf(v1, kv[k + 1], s[k + 1]);
             }
+          }
+          if (K == 64 && !klive) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[k] = 0.f;
           }
           sm.r[quarter][c0 + lane] = column_sums(s, lane);
           {
@@ -585,13 +641,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(tb + tl + cA3 + c0, a);
             tmem_ld32(tb + tl + cA3 + 64 + c0, b);
             tc::tmem_wait_ld();
-            const float end = gate[kGateB + kC - 1];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float v = a[k] + b[k];
-              dk[k] = fmaf(gate[kGateW + c0 + k], v, dk[k]);
-              s[k] = klive ? __expf(end - gate[kGateB + c0 + k]) * v * elem(tq + kTile, c0 + k) : 0.f;
+            for (int k = 0; k < 32; k += 2) {
+              const float2 bw = *reinterpret_cast<const float2*>(gate + kGateW + c0 + k);
+              const float2 wt = *reinterpret_cast<const float2*>(gate + kGateTail + c0 + k);
+              const float v0 = a[k] + b[k], v1 = a[k + 1] + b[k + 1];
+              dk[k] = fmaf(bw.x, v0, dk[k]);
+              dk[k + 1] = fmaf(bw.y, v1, dk[k + 1]);
+              s[k] = wt.x * v0 * kv[k];
+              s[k + 1] = wt.y * v1 * kv[k + 1];
             }
+          }
+          if (K == 64 && !klive) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[k] = 0.f;
           }
           sm.c[quarter][c0 + lane] = column_sums(s, lane);
         }
@@ -620,7 +683,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&bar.qk_empty);  // (its tiles were last read before bar.sums)
       // dq and dk, 32 tokens at a time: through a tile in shared memory to whole 16-byte pieces of their rows
       const int have = min(kC, q.len - tok);
+      uint32_t qo[16], ko[16];
 #pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        qo[k] = pack_pair<__nv_bfloat16>(make_float2(dq[2 * k], dq[2 * k + 1]));
+        ko[k] = pack_pair<__nv_bfloat16>(make_float2(dk[2 * k], dk[2 * k + 1]));
+      }
+#pragma unroll 1
       for (int part = 0; part < 4; ++part) {
         const int which = part >> 1, half = part & 1;
         ok = meet(&bar.epi_sync);  // the tile's last pieces have been read
@@ -628,11 +697,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (klive && hf == half) {
           uint16_t* so = reinterpret_cast<uint16_t*>(smem + lay.out) + row;
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const uint32_t v = which == 0 ? pack_pair<__nv_bfloat16>(make_float2(dq[k], dq[k + 1]))
-                                          : pack_pair<__nv_bfloat16>(make_float2(dk[k], dk[k + 1]));
-            so[k * K] = static_cast<uint16_t>(v);
-            so[(k + 1) * K] = static_cast<uint16_t>(v >> 16);
+          for (int k = 0; k < 16; ++k) {
+            const uint32_t v = which == 0 ? qo[k] : ko[k];
+            so[2 * k * K] = static_cast<uint16_t>(v);
+            so[(2 * k + 1) * K] = static_cast<uint16_t>(v >> 16);
           }
         }
         ok = meet(&bar.epi_sync);

@@ -27,10 +27,6 @@ constexpr int kHeads = 2;   // heads of a group per block
 constexpr int kThreads = 128;
 constexpr int kLd = 68;     // row stride of the fp32 matrices: 16-byte rows, conflict-free fragment reads
 constexpr int kWLd = 20;    // row stride of a warp's 16 x 16 block
-// exp(b_i - b_j) is taken as exp(b_i - b_r) exp(b_r - b_j), r the first token of j's 16-token group, unless the gates
-// of the group sum to more than this (a reset among them)
-constexpr float kWideSpan = 60.f;
-
 struct Matrices {  // over the operand tiles, once their product is read
   float A[kC][kLd];
   float T[kC][kLd];
@@ -199,15 +195,19 @@ __global__ void __launch_bounds__(kThreads, 4) prep_tc_kernel(const __grid_const
       const int t = 2 * lane + k;
       s.b[e][t] = b;
       s.beta[e][t] = be[k];
-      s.key[e][t] = wide ? 1.f : expf(first - b);
+      const float key = wide ? 1.f : expf(first - b), tail = expf(end - b);
+      s.key[e][t] = key;
       rec[kGateE + t] = -expf(b);
-      rec[kGateW + t] = be[k] * expf(end - b);
+      rec[kGateW + t] = be[k] * tail;
       rec[kGateBeta + t] = be[k];
       rec[kGateB + t] = b;
+      rec[kGateKey + t] = key;
+      rec[kGateTail + t] = tail;
     }
     if (lane == 0) {
       rec[kGateEnd] = expf(end);
       s.wide[e] = wb;  // bit 8 g: group g
+      rec[kGateWide] = __uint_as_float(wb);
     }
   }
   tc::fence_before_sync();

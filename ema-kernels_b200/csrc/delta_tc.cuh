@@ -20,10 +20,15 @@ namespace emab {
 namespace delta {
 
 constexpr int kTile = kC * 128;  // bytes of a 64-row, 128-byte-row region
-// gate record of a (chunk, head): -exp(b_i), beta_i exp(b_end - b_i), beta_i, b_i (64 each), exp(b_end)
-constexpr int kGateFloats = 320;
+// gate record of a (chunk, head), 64 each: -exp(b_i), beta_i w_i, beta_i, b_i, key_j = exp(b_r - b_j), w_j = exp(b_end -
+// b_j); then exp(b_end) and, as bits 0, 8, 16, 24 of a word, the wide groups.  exp(b_i - b_j) = exp(b_i - b_r) key_j, r
+// the first token of j's 16-token group, except where a group is wide (its gates sum to more than kWideSpan, a reset
+// among them): there it is taken as it is.
+constexpr float kWideSpan = 60.f;
+constexpr int kGateFloats = 400;
 constexpr uint32_t kStatusTmem = 0x200u;  // device status: a block that owns all of tensor memory did not get base 0
-constexpr int kGateE = 0, kGateW = 64, kGateBeta = 128, kGateB = 192, kGateEnd = 256;
+constexpr int kGateE = 0, kGateW = 64, kGateBeta = 128, kGateB = 192, kGateKey = 256, kGateTail = 320, kGateEnd = 384,
+              kGateWide = 385;
 
 struct TcBuffers {
   float* gates;      // kGateFloats per (slot, head)
@@ -84,7 +89,8 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// A warpgroup's share of the registers the block was launched with; all its warps call it.
+// A warpgroup's share of the registers the block was launched with; all its warps call it.  N is at least (up), at
+// most (down) what it has: the other way round is an illegal instruction.
 template <int N>
 __device__ __forceinline__ void set_regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
