@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -294,6 +295,36 @@ lib.block_norm_workspace_bytes.restype = ctypes.c_size_t
 lib.block_norm_workspace_bytes.argtypes = [_i64] * 3
 lib.ema_last_error.restype = ctypes.c_char_p
 lib.ema_version.restype = ctypes.c_char_p
+
+
+# ---- light launches -----------------------------------------------------------
+# A decoding step's kernels take a few microseconds, so the calls that make one fill their arguments with one
+# struct.pack (the C layout, native alignment) instead of field by field through ctypes.
+
+
+class Launcher:
+    """One launcher of the library: ``Launcher(name, mirror, format)(device_index, *fields)``.
+
+    ``format`` is the struct layout of the ctypes mirror (checked against its size)."""
+
+    def __init__(self, name, mirror, fmt):
+        self.name = name
+        self._pack = struct.Struct("@" + fmt).pack
+        if struct.calcsize("@" + fmt) != ctypes.sizeof(mirror):
+            raise ImportError(f"{name}: struct format and {mirror.__name__} differ in size")
+        self._fn = lib[name]  # a function object of its own: the mirror's stays as declared
+        self._fn.restype = ctypes.c_int
+        self._fn.argtypes = [ctypes.c_char_p, _ptr]
+
+    def __call__(self, index, *fields):
+        args = self._pack(*fields)
+        if torch._C._cuda_getDevice() == index:
+            code = self._fn(args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                code = self._fn(args, torch._C._cuda_getCurrentRawStream(index))
+        if code != EMA_OK:
+            check(code, self.name)
 
 
 class EmaLaunchError(RuntimeError):

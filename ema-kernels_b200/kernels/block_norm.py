@@ -20,11 +20,21 @@ from . import _lib
 __all__ = ["rms_norm_gated", "residual_rms_norm"]
 
 
+_GATED = "3q3if" + "Pq" * 2 + "P" + "Pq" * 4 + "2PN"
+_RESIDUAL = "2q3i2fi" + "Pq" * 2 + "P" + "Pq" * 6 + "2PN"
+_gated_fwd_launch = _lib.Launcher("gated_norm_fwd_launch", _lib.GatedNormArgs, _GATED)
+_gated_bwd_launch = _lib.Launcher("gated_norm_bwd_launch", _lib.GatedNormArgs, _GATED)
+_residual_fwd_launch = _lib.Launcher("residual_norm_fwd_launch", _lib.ResidualNormArgs, _RESIDUAL)
+_residual_bwd_launch = _lib.Launcher("residual_norm_bwd_launch", _lib.ResidualNormArgs, _RESIDUAL)
+_CODES = _lib.DTYPE_CODES
+
+
 def _rows2d(t, dim):
     """t as (rows, dim) with unit channel stride: a view where its strides allow one."""
     if t.ndim != 2:
         t = t.reshape(-1, dim)
-    return t if t.stride(1) == 1 and t.stride(0) >= 0 else t.contiguous()
+    s = t.stride()
+    return t if s[1] == 1 and s[0] >= 0 else t.contiguous()
 
 
 def _workspace(rows, dim, group, dev):
@@ -32,24 +42,13 @@ def _workspace(rows, dim, group, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
-def _gated_args(x, z, weight, eps, group_size, before):
-    a = _lib.GatedNormArgs()
-    a.rows, a.dim, a.group_size = x.shape[0], x.shape[1], group_size
-    a.dtype, a.weight_dtype = _lib.DTYPE_CODES[x.dtype], _lib.DTYPE_CODES[weight.dtype]
-    a.norm_before_gate, a.eps = int(before), eps
-    a.x, a.x_stride, a.z, a.z_stride = x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0)
-    a.weight = weight.data_ptr()
-    return a
-
-
 def _gated_fwd(x, z, weight, eps, group_size, before):
     dim = x.shape[-1]
     x2, z2, w = _rows2d(x, dim), _rows2d(z, dim), weight.contiguous()
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _gated_args(x2, z2, w, eps, group_size, before)
-    a.y, a.y_stride = y.data_ptr(), dim
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib.gated_norm_fwd_launch(a, _lib.stream_ptr(x.device)), "rms_norm_gated")
+    _gated_fwd_launch(x.get_device(), x2.shape[0], dim, group_size, _CODES[x.dtype], _CODES[w.dtype], before, eps,
+                      x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), y.data_ptr(), dim,
+                      0, 0, 0, 0, 0, 0, 0, 0, 0)
     return y
 
 
@@ -58,13 +57,11 @@ def _gated_bwd(x, z, weight, dy, eps, group_size, before):
     x2, z2, w, d2 = _rows2d(x, dim), _rows2d(z, dim), weight.contiguous(), _rows2d(dy.to(x.dtype), dim)
     dx, dz = (torch.empty(x.shape, dtype=x.dtype, device=dev) for _ in range(2))
     dw = torch.empty(dim, dtype=torch.float32, device=dev)
-    a = _gated_args(x2, z2, w, eps, group_size, before)
-    a.dy, a.dy_stride = d2.data_ptr(), d2.stride(0)
-    a.dx, a.dx_stride, a.dz, a.dz_stride, a.dweight = dx.data_ptr(), dim, dz.data_ptr(), dim, dw.data_ptr()
     ws, n = _workspace(x2.shape[0], dim, group_size, dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib.gated_norm_bwd_launch(a, _lib.stream_ptr(dev)), "rms_norm_gated backward")
+    _gated_bwd_launch(x.get_device(), x2.shape[0], dim, group_size, _CODES[x.dtype], _CODES[w.dtype], before, eps,
+                      x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), 0, 0,
+                      d2.data_ptr(), d2.stride(0), dx.data_ptr(), dim, dz.data_ptr(), dim, dw.data_ptr(),
+                      ws.data_ptr(), n)
     return dx, dz, dw
 
 
@@ -105,8 +102,25 @@ def _gated_backward(ctx, dy):
 torch.library.register_autograd("ema_b200::gated_norm_fwd", _gated_backward, setup_context=_gated_setup)
 
 
+class _Gated(torch.autograd.Function):
+    """The eager form of the operators above (torch.compile traces the operators)."""
+
+    @staticmethod
+    def forward(ctx, x, z, weight, eps, group_size, before):
+        ctx.save_for_backward(x, z, weight)
+        ctx.opts = (eps, group_size, before)
+        return _gated_fwd(x, z, weight, eps, group_size, before)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, z, weight = ctx.saved_tensors
+        dx, dz, dw = _gated_bwd(x, z, weight, dy, *ctx.opts)
+        return dx, dz, dw.to(weight.dtype), None, None, None
+
+
 def _check_weight(x, weight, what):
-    if not x.is_cuda or not weight.is_cuda or weight.device != x.device:
+    if not x.is_cuda or weight.device != x.device:
         raise ValueError(f"{what}: the tensors must be on one CUDA device")
     if x.ndim < 1 or x.shape[-1] == 0 or weight.shape != (x.shape[-1],):
         raise ValueError(f"{what}: weight must be ({x.shape[-1] if x.ndim else 0},), got {tuple(weight.shape)}")
@@ -128,34 +142,49 @@ def rms_norm_gated(x, z, weight, eps=1e-5, group_size=None, norm_before_gate=Tru
         raise ValueError(f"rms_norm_gated: group_size {group_size} must divide {dim}")
     if not eps >= 0:
         raise ValueError("rms_norm_gated: eps must not be negative")
-    z = z.to(x.dtype)
-    if torch.compiler.is_compiling() or (
-            torch.is_grad_enabled() and (x.requires_grad or z.requires_grad or weight.requires_grad)):
+    if z.dtype != x.dtype:
+        z = z.to(x.dtype)
+    if torch.compiler.is_compiling():
         return torch.ops.ema_b200.gated_norm_fwd(x, z, weight, float(eps), group_size, bool(norm_before_gate))
+    if torch.is_grad_enabled() and (x.requires_grad or z.requires_grad or weight.requires_grad):
+        return _Gated.apply(x, z, weight, float(eps), group_size, bool(norm_before_gate))
     return _gated_fwd(x, z, weight, float(eps), group_size, bool(norm_before_gate))
 
 
-def _residual_args(rows, dim, dtype, residual_dtype, weight, eps, scale):
-    a = _lib.ResidualNormArgs()
-    a.rows, a.dim, a.eps, a.scale = rows, dim, eps, scale
-    a.dtype, a.residual_dtype = _lib.DTYPE_CODES[dtype], _lib.DTYPE_CODES[residual_dtype]
-    a.weight_dtype, a.weight = _lib.DTYPE_CODES[weight.dtype], weight.data_ptr()
-    return a
+class _Residual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, scale):
+        y, h = _residual_fwd(x, residual, weight, eps, scale)
+        ctx.save_for_backward(weight, h)
+        ctx.has_residual, ctx.x_dtype, ctx.eps, ctx.scale = residual is not None, x.dtype, eps, scale
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        weight, h = ctx.saved_tensors
+        if dy is None and dh is None:
+            return (None,) * 5
+        dy = torch.zeros(h.shape, dtype=ctx.x_dtype, device=h.device) if dy is None else dy.to(ctx.x_dtype)
+        want = ctx.has_residual and ctx.needs_input_grad[1]
+        dx, dr, dw = _residual_bwd(h, weight, dy, dh, ctx.eps, ctx.scale, want)
+        return dx, dr, dw.to(weight.dtype), None, None
 
 
 def _residual_fwd(x, residual, weight, eps, scale):
     dim, dev = x.shape[-1], x.device
-    rdtype = x.dtype if residual is None else residual.dtype
-    x2, r2, w = _rows2d(x, dim), None if residual is None else _rows2d(residual, dim), weight.contiguous()
+    x2, w = _rows2d(x, dim), weight.contiguous()
+    if residual is None:
+        rdtype, rptr, rstride = x.dtype, 0, 0
+    else:
+        r2 = _rows2d(residual, dim)
+        rdtype, rptr, rstride = residual.dtype, r2.data_ptr(), r2.stride(0)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     h = torch.empty(x.shape, dtype=rdtype, device=dev)
-    a = _residual_args(x2.shape[0], dim, x.dtype, rdtype, w, eps, scale)
-    a.x, a.x_stride = x2.data_ptr(), x2.stride(0)
-    if r2 is not None:
-        a.residual, a.residual_stride = r2.data_ptr(), r2.stride(0)
-    a.y, a.y_stride, a.h, a.h_stride = y.data_ptr(), dim, h.data_ptr(), dim
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib.residual_norm_fwd_launch(a, _lib.stream_ptr(dev)), "residual_rms_norm")
+    _residual_fwd_launch(x.get_device(), x2.shape[0], dim, _CODES[x.dtype], _CODES[rdtype], _CODES[w.dtype], eps, scale,
+                         0, x2.data_ptr(), x2.stride(0), rptr, rstride, w.data_ptr(), y.data_ptr(), dim, h.data_ptr(),
+                         dim, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     return y, h
 
 
@@ -165,18 +194,13 @@ def _residual_bwd(h, weight, dy, dh, eps, scale, want_residual):
     dx = torch.empty(h.shape, dtype=dy.dtype, device=dev)
     dr = torch.empty(h.shape, dtype=h.dtype, device=dev) if want_residual else None
     dw = torch.empty(dim, dtype=torch.float32, device=dev)
-    a = _residual_args(h2.shape[0], dim, dy.dtype, h.dtype, w, eps, scale)
-    a.h, a.h_stride, a.dy, a.dy_stride = h2.data_ptr(), h2.stride(0), d2.data_ptr(), d2.stride(0)
     if dh is not None:
         dh = _rows2d(dh.to(h.dtype), dim)
-        a.dh, a.dh_stride = dh.data_ptr(), dh.stride(0)
-    a.dx, a.dx_stride, a.dweight = dx.data_ptr(), dim, dw.data_ptr()
-    if dr is not None:
-        a.d_residual, a.d_residual_stride = dr.data_ptr(), dim
     ws, n = _workspace(h2.shape[0], dim, dim, dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib.residual_norm_bwd_launch(a, _lib.stream_ptr(dev)), "residual_rms_norm backward")
+    _residual_bwd_launch(h.get_device(), h2.shape[0], dim, _CODES[dy.dtype], _CODES[h.dtype], _CODES[w.dtype], eps,
+                         scale, 0, 0, 0, 0, 0, w.data_ptr(), 0, 0, h2.data_ptr(), h2.stride(0), d2.data_ptr(),
+                         d2.stride(0), *((0, 0) if dh is None else (dh.data_ptr(), dh.stride(0))), dx.data_ptr(), dim,
+                         _lib.ptr(dr), dim, dw.data_ptr(), ws.data_ptr(), n)
     return dx, dr, dw
 
 
@@ -241,7 +265,9 @@ def residual_rms_norm(x, residual, weight, eps=1e-5, scale=1.0):
             raise ValueError("residual_rms_norm: the residual has x's type or fp32")
     if not eps >= 0:
         raise ValueError("residual_rms_norm: eps must not be negative")
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and (
-            x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))):
+    if torch.compiler.is_compiling():
         return torch.ops.ema_b200.residual_norm_fwd(x, residual, weight, float(eps), float(scale))
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Residual.apply(x, residual, weight, float(eps), float(scale))
     return _residual_fwd(x, residual, weight, float(eps), float(scale))

@@ -26,13 +26,19 @@ from . import _lib
 
 __all__ = ["gated_delta_rule", "gated_delta_step"]
 
+_T = "P3q"  # a tensor with three strides
+_fwd_launch = _lib.Launcher("delta_fwd_launch", _lib.DeltaFwdArgs, "7qif" + _T * 3 + "4P" + _T + "PPNPN2i")
+_bwd_launch = _lib.Launcher("delta_bwd_launch", _lib.DeltaBwdArgs,
+                            "7qif" + _T * 3 + "3PPN" + _T + "P" + _T * 3 + "3PPN2i")
+_step_launch = _lib.Launcher("delta_step_launch", _lib.DeltaStepArgs, "7qif" + _T * 3 + "3P2qP" + _T)
+
 _DSTATES = (64, 128)
 
 
 def _check(q, k, v, g, beta, what):
-    if not (q.is_cuda and k.is_cuda and v.is_cuda and g.is_cuda and beta.is_cuda):
+    if not v.is_cuda:
         raise ValueError(f"{what}: q, k, v, g and beta must be on CUDA")
-    if not (q.device == k.device == v.device == g.device == beta.device):
+    if not (q.get_device() == k.get_device() == v.get_device() == g.get_device() == beta.get_device()):
         raise ValueError(f"{what}: q, k, v, g and beta must be on one device")
     if v.ndim != 4 or q.ndim != 4:
         raise ValueError(f"{what}: q, k (batch, seqlen, ngroups, dstate), v (batch, seqlen, nheads, headdim)")
@@ -57,57 +63,47 @@ def _check_headdim(V, most, what):
         raise ValueError(f"{what}: headdim must be a multiple of 8 up to {most}, got {V}")
 
 
-def _rows(t):
-    """t itself where its rows can be addressed as they are: unit last stride, 16-byte steps and base."""
+def _rows(t, most=15):
+    """t itself where its rows can be addressed as they are: unit last stride, steps of 16 bytes, a base on 16."""
     es = t.element_size()
-    steps = [s for s, n in zip(t.stride()[:3], t.shape) if n > 1]
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s <= 0 or (s * es) % 16 for s in steps):
-        return t
+    a, b, c, d = t.stride()
+    if d == 1 and not t.data_ptr() & most:
+        n = t.shape
+        if not any(m > 1 and (s <= 0 or (s * es) & 15) for s, m in ((a, n[0]), (b, n[1]), (c, n[2]))):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(t):
+def _strides3(t):
     """Element strides of the three outer axes; an axis of one element, whatever its stride, takes a row's step."""
-    return (_lib._i64 * 3)(*(s if n > 1 else t.shape[3] for s, n in zip(t.stride()[:3], t.shape)))
+    a, b, c, _ = t.stride()
+    n = t.shape
+    return (a if n[0] > 1 else n[3], b if n[1] > 1 else n[3], c if n[2] > 1 else n[3])
 
 
 def _f32(t):
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
-def _set_shape(a, dims, nseq, dtype, scale):
-    a.batch, a.seqlen, a.nheads, a.headdim, a.ngroups, a.dstate = dims
-    a.nseq, a.dtype, a.scale = nseq, _lib.DTYPE_CODES[dtype], scale
-
-
 def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final, save):
     """One forward launch: (o, final states or None, what a backward needs or None)."""
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
-    dims = (b, length, H, V, G, K)
     nseq = b if cu_seqlens is None else cu_seqlens.numel() - 1
-    dev = v.device
+    dev, code = v.device, _lib.DTYPE_CODES[v.dtype]
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), _f32(g), _f32(beta)
     # a packed call's tokens outside every sequence get zeros
     o = (torch.empty if cu_seqlens is None else torch.zeros)(b, length, H, V, dtype=v.dtype, device=dev)
     final = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_final else None
-    a = _lib.DeltaFwdArgs()
-    _set_shape(a, dims, nseq, v.dtype, scale)
-    a.flags = flags
-    size = (b, length, nseq, H, V, K, G, a.dtype, flags)
-    nbytes = _lib.lib.delta_saved_bytes(*size) if save else _lib.lib.delta_workspace_bytes(*size, 0)
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    a.q, a.q_stride, a.k, a.k_stride = q.data_ptr(), _strides(q), k.data_ptr(), _strides(k)
-    a.v, a.v_stride, a.out, a.out_stride = v.data_ptr(), _strides(v), o.data_ptr(), _strides(o)
-    a.g, a.beta, a.cu_seqlens = g.data_ptr(), beta.data_ptr(), _lib.ptr(cu_seqlens)
     s0 = None if initial_states is None else _f32(initial_states)
-    a.initial_states, a.final_states = _lib.ptr(s0), _lib.ptr(final)
-    if save:
-        a.saved, a.saved_bytes = buf.data_ptr(), nbytes
-    else:
-        a.workspace, a.workspace_bytes = buf.data_ptr(), nbytes
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib.delta_fwd_launch(a, _lib.stream_ptr(dev)), "gated_delta_rule")
+    size = (b, length, nseq, H, V, K, G, code, flags)
+    n = _lib.lib.delta_saved_bytes(*size) if save else _lib.lib.delta_workspace_bytes(*size, 0)
+    buf = torch.empty(n, dtype=torch.uint8, device=dev)
+    at = buf.data_ptr()
+    _fwd_launch(v.get_device(), b, length, H, V, K, G, nseq, code, scale, q.data_ptr(), *_strides3(q), k.data_ptr(),
+                *_strides3(k), v.data_ptr(), *_strides3(v), g.data_ptr(), beta.data_ptr(), _lib.ptr(cu_seqlens),
+                _lib.ptr(s0), o.data_ptr(), *_strides3(o), _lib.ptr(final), *((0, 0, at, n) if save else (at, n, 0, 0)),
+                flags, 0)
     return o, final, buf if save else None
 
 
@@ -116,29 +112,22 @@ def _delta_bwd(q, k, v, g, beta, cu_seqlens, saved, do, d_final, scale, flags, w
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
     nseq = b if cu_seqlens is None else cu_seqlens.numel() - 1
-    dev = v.device
+    dev, code = v.device, _lib.DTYPE_CODES[v.dtype]
     q, k, v, g, beta, do = _rows(q), _rows(k), _rows(v), _f32(g), _f32(beta), _rows(do.to(v.dtype))
     new = torch.empty if cu_seqlens is None else torch.zeros
     dq, dk = (new(b, length, G, K, dtype=v.dtype, device=dev) for _ in range(2))
     dv = new(b, length, H, V, dtype=v.dtype, device=dev)
     dg, dbeta = (new(b, length, H, dtype=torch.float32, device=dev) for _ in range(2))
     ds0 = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_d_initial else None
-    a = _lib.DeltaBwdArgs()
-    _set_shape(a, (b, length, H, V, G, K), nseq, v.dtype, scale)
-    a.flags = flags
-    nbytes = _lib.lib.delta_workspace_bytes(b, length, nseq, H, V, K, G, a.dtype, flags, 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    for name, t in (("q", q), ("k", k), ("v", v), ("dout", do), ("dq", dq), ("dk", dk), ("dv", dv)):
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_stride", _strides(t))
-    a.g, a.beta, a.cu_seqlens, a.dg, a.dbeta = (g.data_ptr(), beta.data_ptr(), _lib.ptr(cu_seqlens), dg.data_ptr(),
-                                                dbeta.data_ptr())
-    a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
+    n = _lib.lib.delta_workspace_bytes(b, length, nseq, H, V, K, G, code, flags, 1)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     ds1 = None if d_final is None else _f32(d_final)
-    a.d_final_states, a.d_initial_states = _lib.ptr(ds1), _lib.ptr(ds0)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib.delta_bwd_launch(a, _lib.stream_ptr(dev)), "gated_delta_rule backward")
+    qk, vo = _strides3(dq), _strides3(dv)
+    _bwd_launch(v.get_device(), b, length, H, V, K, G, nseq, code, scale, q.data_ptr(), *_strides3(q), k.data_ptr(),
+                *_strides3(k), v.data_ptr(), *_strides3(v), g.data_ptr(), beta.data_ptr(), _lib.ptr(cu_seqlens),
+                saved.data_ptr(), saved.numel(), do.data_ptr(), *_strides3(do), _lib.ptr(ds1), dq.data_ptr(), *qk,
+                dk.data_ptr(), *qk, dv.data_ptr(), *vo, dg.data_ptr(), dbeta.data_ptr(), _lib.ptr(ds0), ws.data_ptr(),
+                n, flags, 0)
     return dq, dk, dv, dg, dbeta, ds0
 
 
@@ -211,6 +200,32 @@ def _backward(ctx, do, d_final, _d_saved):
 torch.library.register_autograd("ema_b200::delta_fwd", _backward, setup_context=_setup)
 
 
+class _Rule(torch.autograd.Function):
+    """The eager form of the operators above (torch.compile traces the operators)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final):
+        o, final, saved = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final, True)
+        ctx.save_for_backward(q, k, v, g, beta, cu_seqlens, saved)
+        ctx.scale, ctx.flags = scale, flags
+        ctx.initial_dtype = None if initial_states is None else initial_states.dtype
+        ctx.set_materialize_grads(False)
+        return o, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, d_final):
+        q, k, v, g, beta, cu, saved = ctx.saved_tensors
+        if do is None and d_final is None:
+            return (None,) * 10
+        if do is None:
+            do = torch.zeros_like(v)
+        want = ctx.initial_dtype is not None and ctx.needs_input_grad[5]
+        dq, dk, dv, dg, dbeta, ds0 = _delta_bwd(q, k, v, g, beta, cu, saved, do, d_final, ctx.scale, ctx.flags, want)
+        return (dq, dk, dv, dg.to(g.dtype), dbeta.to(beta.dtype), ds0.to(ctx.initial_dtype) if want else None,
+                None, None, None, None)
+
+
 def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_final_states=False, cu_seqlens=None,
                      fp32_products=False):
     """o (batch, seqlen, nheads, headdim), or (o, final states) with ``return_final_states``.
@@ -244,11 +259,11 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
                              f"{tuple(initial_states.shape)}")
     scale = K ** -0.5 if scale is None else float(scale)
     flags = _lib.DELTA_FP32_PRODUCTS if fp32_products else 0
-    wants = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states))
-    if wants or torch.compiler.is_compiling():
-        o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale,
-                                                   flags)
+    if torch.compiler.is_compiling():
+        o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags)
+    elif torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states)):
+        o, final = _Rule.apply(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, return_final_states)
     else:
         o, final, _ = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, return_final_states,
                                  False)
@@ -261,16 +276,11 @@ def _delta_step(q, k, v, g, beta, states, state_indices, scale):
     q, k, g, beta = _rows(q), _rows(k), _f32(g), _f32(beta)
     if v.stride(3) != 1:
         v = v.clone(memory_format=torch.contiguous_format)
-    a = _lib.DeltaStepArgs()
-    a.batch, a.tokens, a.nheads, a.headdim, a.dstate, a.ngroups = b, T, H, V, q.shape[3], q.shape[2]
-    a.slots, a.dtype, a.scale = states.shape[0], _lib.DTYPE_CODES[v.dtype], scale
-    a.q, a.q_stride, a.k, a.k_stride = q.data_ptr(), _strides(q), k.data_ptr(), _strides(k)
-    a.v, a.v_stride, a.out, a.out_stride = v.data_ptr(), _strides(v), o.data_ptr(), _strides(o)
-    a.g, a.beta, a.states, a.state_indices = (g.data_ptr(), beta.data_ptr(), states.data_ptr(),
-                                              _lib.ptr(state_indices))
-    a.state_stride = (_lib._i64 * 2)(states.stride(0), states.stride(1))
-    with torch.cuda.device(v.device):
-        _lib.check(_lib.lib.delta_step_launch(a, _lib.stream_ptr(v.device)), "gated_delta_step")
+    ss = states.stride()
+    _step_launch(v.get_device(), b, T, H, V, q.shape[3], q.shape[2], states.shape[0], _lib.DTYPE_CODES[v.dtype], scale,
+                 q.data_ptr(), *_strides3(q), k.data_ptr(), *_strides3(k), v.data_ptr(), *_strides3(v), g.data_ptr(),
+                 beta.data_ptr(), states.data_ptr(), ss[0], ss[1], _lib.ptr(state_indices), o.data_ptr(), T * H * V,
+                 H * V, V)
     return o
 
 
@@ -298,28 +308,31 @@ def gated_delta_step(q, k, v, g, beta, states, scale=None, state_indices=None):
         q, k, v, g, beta = (t.unsqueeze(1) for t in (q, k, v, g, beta))
     b, _, H, V, _, K = _check(q, k, v, g, beta, "gated_delta_step")
     _check_headdim(V, 256, "gated_delta_step")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, states)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or beta.requires_grad or states.requires_grad):
         raise ValueError("gated_delta_step has no gradient: call it under torch.no_grad() or use gated_delta_rule")
-    if states.ndim != 4 or states.shape[1:] != (H, V, K) or states.dtype != torch.float32:
+    if states.shape[1:] != (H, V, K) or states.dtype != torch.float32:
         raise ValueError(f"gated_delta_step: states must be (slots, {H}, {V}, {K}) fp32, got {tuple(states.shape)} "
                          f"{states.dtype}")
-    if states.device != v.device:
+    if states.get_device() != v.get_device():
         raise ValueError("gated_delta_step: states must be on v's device")
-    if states.stride(3) != 1 or states.stride(2) != K or states.data_ptr() % 16 or any(
-            s % 4 for s in states.stride()[:2]):
-        raise ValueError("gated_delta_step: the (headdim, dstate) block of a state must be contiguous, 16-byte aligned")
+    s0, s1, s2, s3 = states.stride()
+    if s3 != 1 or s2 != K or states.data_ptr() & 15 or (s0 | s1) & 3 or (
+            states.shape[0] > 1 and s0 < V * K) or (H > 1 and s1 < V * K):
+        raise ValueError("gated_delta_step: the (headdim, dstate) block of a state must be contiguous, 16-byte aligned "
+                         "and its own")
     if state_indices is None:
         if states.shape[0] < b:
             raise ValueError(f"gated_delta_step: {b} rows on {states.shape[0]} slots")
     else:
         if state_indices.shape != (b,) or state_indices.dtype not in (torch.int32, torch.int64):
             raise ValueError("gated_delta_step: state_indices must be (batch,) int32 or int64")
-        if state_indices.device != v.device:
+        if state_indices.get_device() != v.get_device():
             raise ValueError("gated_delta_step: state_indices must be on v's device")
         if state_indices.dtype == torch.int64:
             # clamped before the narrowing, so that a huge index stays outside the cache
-            state_indices = state_indices.clamp(-1, states.shape[0])
-        state_indices = state_indices.to(torch.int32).contiguous()
+            state_indices = state_indices.clamp(-1, states.shape[0]).to(torch.int32)
+        state_indices = state_indices.contiguous()
     scale = K ** -0.5 if scale is None else float(scale)
     if torch.compiler.is_compiling():
         o = torch.ops.ema_b200.delta_step(q, k, v, g, beta, states, state_indices, scale)
