@@ -25,6 +25,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "block_norm_b200.h"
 #include "ema_common.cuh"
@@ -55,7 +56,8 @@ struct Params {
   float* partial;  // (blocks, m) of this group's weight gradient, group-major
 };
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+// (the approximate reciprocal is within 2 ulp, and 0 where exp(-v) overflows)
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
 __device__ __forceinline__ float load_weight(const void* w, int type, int i) {
   if (type == EMA_DTYPE_F32) return static_cast<const float*>(w)[i];
@@ -63,20 +65,21 @@ __device__ __forceinline__ float load_weight(const void* w, int type, int i) {
   return to_f32(static_cast<const __half*>(w)[i]);
 }
 
-// VEC consecutive elements; `al`: all rows of the call start on 16 bytes (uniform over the grid).
+// VEC consecutive elements as they lie in memory; `al`: all rows of the call start on 16 bytes (uniform over the grid).
 template <class T, int VEC>
-__device__ __forceinline__ void load_v(const T* p, bool al, float (&f)[VEC]) {
+struct alignas(sizeof(T) * VEC >= 16 ? 16 : sizeof(T) * VEC) Raw {
+  T e[VEC];
+};
+template <class T, int VEC>
+__device__ __forceinline__ void load_raw(const void* base, long long at, bool al, Raw<T, VEC>& r) {
+  const T* p = static_cast<const T*>(base) + at;
   if (VEC == 1 || !al) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) f[k] = to_f32(p[k]);
-  } else if constexpr (VEC == 8) {
-    float2 v[4];
-    load8<T>(p, v);
+    for (int k = 0; k < VEC; ++k) r.e[k] = p[k];
+  } else {
+    uint4* to = reinterpret_cast<uint4*>(&r);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f[2 * k] = v[k].x;
-      f[2 * k + 1] = v[k].y;
-    }
+    for (int k = 0; k < static_cast<int>(sizeof(r) / 16); ++k) to[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
   }
 }
 template <class T, int VEC>
@@ -147,13 +150,21 @@ __device__ __forceinline__ void write_partial(const Params& p, const float (&dw)
   }
 }
 
-// grid: (row blocks, groups of a row).  One norm row per group of TG threads and iteration.
-template <class T, class R, int TG, int VEC, int NV, bool RES, bool BWD>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const Params p) {
+// grid: (row blocks, groups of a row).  One norm row per group of TG threads and iteration; the next row's loads are
+// issued before this one's arithmetic (raw, so a 16-bit tensor costs four registers a vector), which is what keeps enough
+// bytes in flight: without it the gated pair at 8192 x 32 heads of 128 took 202 and 396 us, see the table of cases.
+// FIRST: the norm comes before the gate.
+template <class T, class R, int TG, int VEC, int NV, bool RES, bool BWD, bool FIRST>
+__global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? (BWD ? 2 : 3) : 1) norm_kernel(const Params p) {
   __shared__ float2 buf[2][kThreads / 32];
+  using TA = std::conditional_t<RES && BWD, R, T>;  // x, or h
+  using TB = std::conditional_t<RES, R, T>;         // the gate, the residual, or dh
   const int lane = threadIdx.x % TG, grp = threadIdx.x / TG;
   const int g0 = blockIdx.y * p.m;
   const float inv_m = 1.f / static_cast<float>(p.m);
+  const void* pa = RES && BWD ? p.h : p.x;
+  const void* pb = RES && BWD ? p.dh : p.z;
+  const long long sa = RES && BWD ? p.sh : p.sx, sb = RES && BWD ? p.sdh : p.sz;
   int turn = 0;
   float w[NV][VEC], dw[NV][VEC];
 #pragma unroll
@@ -165,43 +176,56 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const Params p) {
       dw[j][k] = 0.f;
     }
   constexpr int NG = kThreads / TG;
+  // (long rows have enough bytes in flight by themselves, and no registers for two)
+  constexpr bool kAhead = NV * VEC * static_cast<int>(sizeof(T)) <= 32;
   const long long step = static_cast<long long>(gridDim.x) * NG;
+  Raw<TA, VEC> ra[NV];
+  Raw<TB, VEC> rb[NV];
+  Raw<T, VEC> rc[NV];
+  auto fetch = [&](long long row, Raw<TA, VEC> (&a)[NV], Raw<TB, VEC> (&b)[NV], Raw<T, VEC> (&d)[NV]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TG + lane) * VEC;
+      if (row < p.rows && c < p.m) {
+        load_raw<TA, VEC>(pa, row * sa + g0 + c, p.aligned, a[j]);
+        if (!RES || pb != nullptr) load_raw<TB, VEC>(pb, row * sb + g0 + c, p.aligned, b[j]);
+        if (BWD) load_raw<T, VEC>(p.dy, row * p.sdy + g0 + c, p.aligned, d[j]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) a[j].e[k] = from_f32<TA>(0.f), b[j].e[k] = from_f32<TB>(0.f), d[j].e[k] = from_f32<T>(0.f);
+      }
+      if (RES && pb == nullptr)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) b[j].e[k] = from_f32<TB>(0.f);
+    }
+  };
+  if (kAhead) fetch(static_cast<long long>(blockIdx.x) * NG + grp, ra, rb, rc);
   // every thread of a warp takes part in the shuffles of every iteration: a group without a row adds zeros
   for (long long r0 = static_cast<long long>(blockIdx.x) * NG; r0 < p.rows; r0 += step) {
     const long long row = r0 + grp;
     const bool live = row < p.rows;
-    float t[NV][VEC], z[NV][VEC], d[NV][VEC];
+    Raw<TA, VEC> na[NV];
+    Raw<TB, VEC> nb[NV];
+    Raw<T, VEC> nd[NV];
+    if (!kAhead) fetch(row, ra, rb, rc);
+    else if (r0 + step < p.rows) fetch(row + step, na, nb, nd);
+    float t[NV][VEC], sg[NV][VEC];  // the normed value, the gate's sigmoid
     float sum = 0.f, dot = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * TG + lane) * VEC;
-      const bool in = live && c < p.m;
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) t[j][k] = z[j][k] = d[j][k] = 0.f;
-      if (in) {
-        if (!(RES && BWD)) load_v<T, VEC>(static_cast<const T*>(p.x) + row * p.sx + g0 + c, p.aligned, t[j]);
-        if (RES && BWD) load_v<R, VEC>(static_cast<const R*>(p.h) + row * p.sh + g0 + c, p.aligned, t[j]);
-        if (!RES) load_v<T, VEC>(static_cast<const T*>(p.z) + row * p.sz + g0 + c, p.aligned, z[j]);
-        if (RES && !BWD && p.z != nullptr)
-          load_v<R, VEC>(static_cast<const R*>(p.z) + row * p.sz + g0 + c, p.aligned, z[j]);
-        if (BWD) load_v<T, VEC>(static_cast<const T*>(p.dy) + row * p.sdy + g0 + c, p.aligned, d[j]);
-        if (RES && BWD && p.dh != nullptr)
-          load_v<R, VEC>(static_cast<const R*>(p.dh) + row * p.sdh + g0 + c, p.aligned, z[j]);
-      }
-    }
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
+        const float a = to_f32(ra[j].e[k]), z = to_f32(rb[j].e[k]), d = BWD ? to_f32(rc[j].e[k]) : 0.f;
         if (RES) {
-          if (!BWD) t[j][k] = to_f32(from_f32<R>(fmaf(p.scale, t[j][k], z[j][k])));
+          t[j][k] = BWD ? a : to_f32(from_f32<R>(fmaf(p.scale, a, z)));
           sum = fmaf(t[j][k], t[j][k], sum);
-          if (BWD) dot = fmaf(d[j][k] * w[j][k], t[j][k], dot);
+          if (BWD) dot = fmaf(d * w[j][k], t[j][k], dot);
         } else {
-          const float s = z[j][k] * sigmoid(z[j][k]);
-          const float v = p.before ? t[j][k] : t[j][k] * s;
-          sum = fmaf(v, v, sum);
-          if (BWD) dot = fmaf((p.before ? d[j][k] * s : d[j][k]) * w[j][k], v, dot);
+          sg[j][k] = sigmoid(z);
+          const float s = z * sg[j][k];
+          t[j][k] = FIRST ? a : a * s;
+          sum = fmaf(t[j][k], t[j][k], sum);
+          if (BWD) dot = fmaf((FIRST ? d * s : d) * w[j][k], t[j][k], dot);
         }
       }
     const float2 sums = group_sum<TG>(sum, dot, buf, turn);
@@ -213,26 +237,26 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const Params p) {
       float a[VEC], b[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
+        const float z = to_f32(rb[j].e[k]), d = BWD ? to_f32(rc[j].e[k]) : 0.f;
+        const float th = t[j][k] * rstd;
         if (RES) {
-          const float th = t[j][k] * rstd;
           if (!BWD) {
             a[k] = th * w[j][k];
           } else {
-            b[k] = fmaf(rstd, fmaf(-th, c1, d[j][k] * w[j][k]), z[j][k]);
+            b[k] = fmaf(rstd, fmaf(-th, c1, d * w[j][k]), z);
             a[k] = p.scale * b[k];
-            dw[j][k] = fmaf(d[j][k], th, dw[j][k]);
+            dw[j][k] = fmaf(d, th, dw[j][k]);
           }
         } else {
-          const float sg = sigmoid(z[j][k]), s = z[j][k] * sg;
-          const float th = (p.before ? t[j][k] : t[j][k] * s) * rstd;
+          const float s = z * sg[j][k];
           if (!BWD) {
-            a[k] = th * w[j][k] * (p.before ? s : 1.f);
+            a[k] = th * w[j][k] * (FIRST ? s : 1.f);
           } else {
-            const float ds = sg * (1.f + z[j][k] * (1.f - sg));
-            const float dn = p.before ? d[j][k] * s : d[j][k];
+            const float ds = sg[j][k] * (1.f + z * (1.f - sg[j][k]));
+            const float dn = FIRST ? d * s : d;
             const float dt = rstd * fmaf(-th, c1, dn * w[j][k]);
-            a[k] = p.before ? dt : dt * s;
-            b[k] = p.before ? d[j][k] * th * w[j][k] * ds : dt * t[j][k] * ds;
+            a[k] = FIRST ? dt : dt * s;
+            b[k] = FIRST ? d * th * w[j][k] * ds : dt * to_f32(ra[j].e[k]) * ds;
             dw[j][k] = fmaf(dn, th, dw[j][k]);
           }
         }
@@ -246,6 +270,11 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const Params p) {
           if (!RES) store_v<T, VEC>(static_cast<T*>(p.dz) + row * p.sdz + g0 + c, p.aligned, b);
           if (RES && p.dz != nullptr) store_v<R, VEC>(static_cast<R*>(p.dz) + row * p.sdz + g0 + c, p.aligned, b);
         }
+      }
+      if (kAhead) {
+        ra[j] = na[j];
+        rb[j] = nb[j];
+        if (BWD) rc[j] = nd[j];
       }
     }
   }
@@ -323,23 +352,23 @@ __global__ void __launch_bounds__(kThreads) norm_wide_kernel(const Params p) {
   }
 }
 
-// dweight[group][c] = sum over the blocks of partial[group][block][c].  A block owns 32 columns; its eight
-// warps take every eighth row of partials and are joined in shared memory in warp order.
-__global__ void __launch_bounds__(256) weight_grad_kernel(const float* partial, float* dw, int m, int blocks) {
-  __shared__ float s[8][32];
+// dweight[group][c] = sum over the blocks of partial[group][block][c].  A block owns 32 columns; its 32 warps take
+// every 32nd row of partials, eight in flight, and are joined in shared memory in warp order.
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* partial, float* dw, int m, int blocks) {
+  __shared__ float s[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const float* src = partial + static_cast<long long>(blockIdx.y) * blocks * m;
   float v = 0.f;
   if (c < m) {
-#pragma unroll 4
-    for (int b = warp; b < blocks; b += 8) v += src[static_cast<long long>(b) * m + c];
+#pragma unroll 8
+    for (int b = warp; b < blocks; b += 32) v += src[static_cast<long long>(b) * m + c];
   }
   s[warp][lane] = v;
   __syncthreads();
   if (warp == 0 && c < m) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += s[i][lane];
+    for (int i = 1; i < 32; ++i) v += s[i][lane];
     dw[static_cast<long long>(blockIdx.y) * m + c] = v;
   }
 }
@@ -377,34 +406,29 @@ Layout layout(int64_t m) {
 }
 // Blocks over the rows of one group: enough for every SM to hold several, no more than there are rows.
 int64_t row_blocks(int64_t rows, int64_t groups, int per_block) {
-  constexpr int64_t kTarget = 148 * 4;
+  constexpr int64_t kTarget = 148 * 6;
   int64_t want = (kTarget + groups - 1) / groups;
   const int64_t have = (rows + per_block - 1) / per_block;
   if (want > have) want = have;
   return want < 1 ? 1 : want;
 }
 
+template <class T, class R, bool RES, bool BWD, bool FIRST>
+void run_rows(const Params& p, const Layout& l, dim3 grid, cudaStream_t st) {
+  if (!l.vec) norm_kernel<T, R, 256, 1, 8, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else if (l.tg == 8) norm_kernel<T, R, 8, 8, 1, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else if (l.tg == 16) norm_kernel<T, R, 16, 8, 1, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else if (l.tg == 32 && l.nv == 1) norm_kernel<T, R, 32, 8, 1, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else if (l.tg == 32) norm_kernel<T, R, 32, 8, 2, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else if (l.nv == 1) norm_kernel<T, R, 256, 8, 1, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else if (l.nv == 2) norm_kernel<T, R, 256, 8, 2, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+  else norm_kernel<T, R, 256, 8, 4, RES, BWD, FIRST><<<grid, kThreads, 0, st>>>(p);
+}
 template <class T, class R, bool RES, bool BWD>
 void run(const Params& p, const Layout& l, dim3 grid, cudaStream_t st) {
-  if (l.wide) {
-    norm_wide_kernel<T, R, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (!l.vec) {
-    norm_kernel<T, R, 256, 1, 8, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (l.tg == 8) {
-    norm_kernel<T, R, 8, 8, 1, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (l.tg == 16) {
-    norm_kernel<T, R, 16, 8, 1, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (l.tg == 32 && l.nv == 1) {
-    norm_kernel<T, R, 32, 8, 1, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (l.tg == 32) {
-    norm_kernel<T, R, 32, 8, 2, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (l.nv == 1) {
-    norm_kernel<T, R, 256, 8, 1, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else if (l.nv == 2) {
-    norm_kernel<T, R, 256, 8, 2, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  } else {
-    norm_kernel<T, R, 256, 8, 4, RES, BWD><<<grid, kThreads, 0, st>>>(p);
-  }
+  if (l.wide) norm_wide_kernel<T, R, RES, BWD><<<grid, kThreads, 0, st>>>(p);
+  else if (!RES && p.before) run_rows<T, R, RES, BWD, !RES>(p, l, grid, st);
+  else run_rows<T, R, RES, BWD, false>(p, l, grid, st);
 }
 
 template <bool RES, bool BWD>
@@ -435,7 +459,7 @@ int launch(Params& p, int dtype, int rtype, bool vec, float* dweight, void* ws, 
     else run<__half, float, RES, BWD>(p, l, grid, st);
   }
   if (BWD)
-    weight_grad_kernel<<<dim3(static_cast<unsigned>((p.m + 31) / 32), static_cast<unsigned>(groups)), 256, 0, st>>>(
+    weight_grad_kernel<<<dim3(static_cast<unsigned>((p.m + 31) / 32), static_cast<unsigned>(groups)), 1024, 0, st>>>(
         p.partial, dweight, p.m, static_cast<int>(blocks));
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(EMA_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));

@@ -308,14 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       unsigned char* base = smem + st * St::kBytes;
       const float* gate = reinterpret_cast<const float*>(base + St::oG);
       const long long ch = static_cast<long long>(q.slot + c) * p.H + h;
-      {  // dS as hi / lo operand columns, and as the image of this chunk's end
-        if (row < VP) {
-          float* img = w.dS + ch * state_image(p.V, K);
-#pragma unroll
-          for (int i = 0; i < KC / 4; ++i)
-            *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
-                make_float4(D[2 * i].x, D[2 * i].y, D[2 * i + 1].x, D[2 * i + 1].y);
-        }
+      {  // dS as hi / lo operand columns
 #pragma unroll
         for (int g = 0; g < KC / 32; ++g) {
           uint32_t hi[16], lo[16];
@@ -327,6 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
       }
       arrive(&bar.s);
+      if (row < VP) {
+        float* img = w.dS + ch * state_image(p.V, K);
+#pragma unroll
+        for (int i = 0; i < KC / 4; ++i)
+          *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
+              make_float4(D[2 * i].x, D[2 * i].y, D[2 * i + 1].x, D[2 * i + 1].y);
+      }
       if (!wait(&bar.full[st], (r / kStages) & 1) || !wait(&bar.z, r & 1)) break;
       tc::fence_after_sync();
       float2 x[16];  // W, then dX

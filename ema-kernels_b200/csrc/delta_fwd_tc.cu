@@ -322,16 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
-    // the state as hi / lo operand columns, and as the image of the chunk it enters
-    auto publish = [&](int c) {
-      const long long ch = static_cast<long long>(q.slot + c) * p.H + h;
-      if (KEEP && row < VP) {
-        float* img = w.S + ch * state_image(p.V, K);
-#pragma unroll
-        for (int i = 0; i < KC / 4; ++i)
-          *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
-              make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
-      }
+    // the state as hi / lo operand columns
+    auto publish = [&]() {
 #pragma unroll
       for (int g = 0; g < KC / 32; ++g) {
         uint32_t hi[16], lo[16];
@@ -343,8 +335,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::tmem_wait_st();
     };
     for (int c = 0; c < nc; ++c) {
-      publish(c);
+      publish();
       arrive(&bar.s);
+      if (KEEP && row < VP) {
+        float* img = w.S + (static_cast<long long>(q.slot + c) * p.H + h) * state_image(p.V, K);
+#pragma unroll
+        for (int i = 0; i < KC / 4; ++i)
+          *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
+              make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
+      }
       const int st = c % kStages;
       const unsigned char* base = smem + st * St::kBytes;
       const float* gate = reinterpret_cast<const float*>(base + St::oG);
