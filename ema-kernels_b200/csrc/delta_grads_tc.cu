@@ -37,7 +37,7 @@ namespace {
 constexpr int kEpi = 8, kAux = 4;
 constexpr int kMma = 12, kLoad = 13, kGates = 14;  // (15 only fills its warpgroup)
 constexpr int kThreads = 16 * 32;
-constexpr int kRegEpi = 160, kRegAux = 136, kRegCtl = 56;
+constexpr int kRegEpi = 152, kRegAux = 128, kRegCtl = 80;
 static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128 && kRegAux >= 128 && kRegCtl <= 128, "register split");
 constexpr int kRing = 2;
 constexpr int kReg = 128 * 128;  // two 64-row tiles of 64 columns, one over the other
@@ -108,29 +108,18 @@ __device__ __forceinline__ void stage_lo8(unsigned char* to, const float2 (&v)[4
   *reinterpret_cast<uint4*>(to) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// Column sums over the warp's 32 lanes: lane l gets column l.
-__device__ __forceinline__ float column_sums(float (&x)[32], int lane) {
+// Sums of 16 columns over the warp's 32 lanes: lane l gets column l / 2.
+__device__ __forceinline__ float column_sums(float (&x)[16], int lane) {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
+  for (int o = 16, n = 8; n >= 1; o >>= 1, n >>= 1) {
     const bool up = (lane & o) != 0;
 #pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float give = up ? x[i] : x[i + o];
-      x[i] = (up ? x[i + o] : x[i]) + __shfl_xor_sync(0xffffffffu, give, o);
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? x[i] : x[i + n];
+      x[i] = (up ? x[i + n] : x[i]) + __shfl_xor_sync(0xffffffffu, give, o);
     }
   }
-  return x[0];
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t at, float (&v)[32]) {
-  float a[16], b[16];
-  tc::tmem_ld16(at, a);
-  tc::tmem_ld16(at + 16, b);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    v[i] = a[i];
-    v[16 + i] = b[i];
-  }
+  return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 1);
 }
 
 template <int K>
@@ -232,22 +221,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idMM128 = tc::idesc_bf16(128, 128, true, true);
       constexpr uint32_t idMM = tc::idesc_bf16(128, 64, true, true);
       constexpr uint32_t idMK = tc::idesc_bf16(128, 64, true, false);
-      auto kstep = [](int s) { return static_cast<uint64_t>(((s >> 2) * kReg + (s & 3) * 32) >> 4); };
-      auto nstep = [](int s) { return static_cast<uint64_t>((s * 2048) >> 4); };
-      auto jstep = [](int s) { return static_cast<uint64_t>((s * 32) >> 4); };
+      auto kstep = [](int s) { return static_cast<uint32_t>(((s >> 2) * kReg + (s & 3) * 32) >> 4); };
+      auto nstep = [](int s) { return static_cast<uint32_t>((s * 2048) >> 4); };
+      auto jstep = [](int s) { return static_cast<uint32_t>((s * 32) >> 4); };
       const uint32_t sb = smem_u32(smem);
       // state columns as lanes: two 64-column regions (dstate 64: the same one twice, the upper lanes are not read)
       constexpr uint32_t sreg = K == 128 ? 2048u : 0u, qreg = K == 128 ? kReg : 0u;
-      const uint64_t dQK = tc::smem_desc_sw128(sb, 16, 1024), dK = tc::smem_desc_sw128(sb + kTile, 16, 1024);
-      const uint64_t dQn = tc::smem_desc_sw128(sb, qreg, 1024), dKn = tc::smem_desc_sw128(sb + kTile, qreg, 1024);
-      const uint64_t dOX = tc::smem_desc_sw128(sb + lay.ox, 16, 1024);
-      const uint64_t dE = tc::smem_desc_sw128(sb + lay.ex, img, 1024);            // [E hi | E mid]
-      const uint64_t dEm = tc::smem_desc_sw128(sb + lay.ex + img, img, 1024);     // E mid
-      const uint64_t dEl = tc::smem_desc_sw128(sb + lay.ex + 2 * img, img, 1024); // E lo
-      const uint64_t dEX = tc::smem_desc_sw128(sb + lay.ex, 3 * img, 1024);       // [E hi | dX lo]
-      const uint64_t dXl = tc::smem_desc_sw128(sb + lay.ex + 3 * img, img, 1024);
-      const uint64_t dN = tc::smem_desc_sw128(sb + lay.nm, 16, 1024), dM = tc::smem_desc_sw128(sb + lay.nm + kTile, 16, 1024);
-      const uint64_t dNl = tc::smem_desc_sw128(sb + lay.out, 16, 1024);
+      const uint32_t dQK = desc_lo(sb, 16), dK = desc_lo(sb + kTile, 16);
+      const uint32_t dQn = desc_lo(sb, qreg), dKn = desc_lo(sb + kTile, qreg);
+      const uint32_t dOX = desc_lo(sb + lay.ox, 16);
+      const uint32_t dE = desc_lo(sb + lay.ex, img);            // [E hi | E mid]
+      const uint32_t dEm = desc_lo(sb + lay.ex + img, img);     // E mid
+      const uint32_t dEl = desc_lo(sb + lay.ex + 2 * img, img); // E lo
+      const uint32_t dEX = desc_lo(sb + lay.ex, 3 * img);       // [E hi | dX lo]
+      const uint32_t dXl = desc_lo(sb + lay.ex + 3 * img, img);
+      const uint32_t dRing = desc_lo(sb + lay.ring, sreg);
+      const uint32_t dN = desc_lo(sb + lay.nm, 16), dM = desc_lo(sb + lay.nm + kTile, 16);
+      const uint32_t dNl = desc_lo(sb + lay.out, 16);
       int n, tok, task = 0, hc = 0, rc = 0;
       Seq q;
       bool ok = true;
@@ -281,57 +271,67 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) {
             if (h == 0) {
 #pragma unroll 1
-              for (int s = 0; s < K / 16; ++s) tc::mma_bf16(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
+              for (int s = 0; s < K / 16; ++s) mma_ss(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
             }
 #pragma unroll 1
-            for (int s = 0; s < steps; ++s) {
-              tc::mma_bf16(tb + cF, dOX + kstep(s), dE + nstep(s), idF, s > 0);
-              tc::mma_bf16(tb + cF, dOX + kstep(s), dEl + nstep(s), idF64, true);
-              tc::mma_bf16(tb + cF + 128, dEX + nstep(s), dE + nstep(s), idMM, s > 0);
-              tc::mma_bf16(tb + cF + 128, dEX + nstep(s), dEm + nstep(s), idMM, true);
+            for (int s4 = 0; s4 < steps / 4; ++s4) {  // 64 value channels
+              const uint32_t ox = dOX + s4 * (kReg >> 4), vo = static_cast<uint32_t>(s4 * 512);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const bool more = s4 > 0 || i > 0;
+                mma_ss(tb + cF, ox + 2 * i, dE + vo + 128 * i, idF, more);
+                mma_ss(tb + cF, ox + 2 * i, dEl + vo + 128 * i, idF64, true);
+                mma_ss(tb + cF + 128, dEX + vo + 128 * i, dE + vo + 128 * i, idMM, more);
+                mma_ss(tb + cF + 128, dEX + vo + 128 * i, dEm + vo + 128 * i, idMM, true);
+              }
             }
             tc::mma_commit(&bar.f);
           }
           __syncwarp();
 #pragma unroll 1
-          for (int s = 0; s < steps; ++s, ++rc) {
-            const int st = rc % kRing;
-            ok = wait(&bar.s_full[st], (rc / kRing) & 1);
-            if (!ok) break;
-            const uint32_t at = sb + lay.ring + st * Layout<K>::kStep;
-            constexpr uint64_t pc = Layout<K>::kPiece >> 4;
-            const uint64_t dS = tc::smem_desc_sw128(at, sreg, 1024), dD = tc::smem_desc_sw128(at + 3 * Layout<K>::kPiece, sreg, 1024);
-            if (elect_one()) {
-              tc::mma_bf16(tb + cA, dS, dOX + kstep(s), idA, s > 0);
-              tc::mma_bf16(tb + cA, dS + pc, dOX + kstep(s), idA, true);
-              tc::mma_bf16(tb + cA, dS + 2 * pc, dOX + kstep(s), idA, true);
-              tc::mma_bf16(tb + cA + 64, dS, dXl + nstep(s), idMM, true);
-              tc::mma_bf16(tb + cA + 64, dS + pc, dXl + nstep(s), idMM, true);
-              tc::mma_bf16(tb + cA3, dD, dE + nstep(s), idMM128, s > 0);
-              tc::mma_bf16(tb + cA3, dD + pc, dE + nstep(s), idMM128, true);
-              tc::mma_bf16(tb + cA3, dD, dEl + nstep(s), idMM, true);
-              tc::mma_bf16(tb + cA3, dD + 2 * pc, dE + nstep(s), idMM, true);
-              tc::mma_commit(&bar.s_empty[st]);
-              if (s == steps - 1) {
-                tc::mma_commit(&bar.a);
-                tc::mma_commit(&bar.ox_empty);
-                tc::mma_commit(&bar.ex_empty);
+          for (int s4 = 0; ok && s4 < steps / 4; ++s4) {
+            const uint32_t ox = dOX + s4 * (kReg >> 4), vo = static_cast<uint32_t>(s4 * 512);
+#pragma unroll
+            for (int i = 0; i < 4; ++i, ++rc) {  // (steps is a multiple of the ring: step i uses slot i % kRing)
+              const int st = i % kRing;
+              ok = ok && wait(&bar.s_full[st], (rc / kRing) & 1);
+              if (!ok) break;
+              constexpr uint32_t pc = Layout<K>::kPiece >> 4;
+              const uint32_t dS = dRing + st * (Layout<K>::kStep >> 4), dD = dS + 3 * pc;
+              if (elect_one()) {
+                const bool more = s4 > 0 || i > 0;
+                mma_ss(tb + cA, dS, ox + 2 * i, idA, more);
+                mma_ss(tb + cA, dS + pc, ox + 2 * i, idA, true);
+                mma_ss(tb + cA, dS + 2 * pc, ox + 2 * i, idA, true);
+                mma_ss(tb + cA + 64, dS, dXl + vo + 128 * i, idMM, true);
+                mma_ss(tb + cA + 64, dS + pc, dXl + vo + 128 * i, idMM, true);
+                mma_ss(tb + cA3, dD, dE + vo + 128 * i, idMM128, more);
+                mma_ss(tb + cA3, dD + pc, dE + vo + 128 * i, idMM128, true);
+                mma_ss(tb + cA3, dD, dEl + vo + 128 * i, idMM, true);
+                mma_ss(tb + cA3, dD + 2 * pc, dE + vo + 128 * i, idMM, true);
+                tc::mma_commit(&bar.s_empty[st]);
               }
+              __syncwarp();
             }
-            __syncwarp();
           }
           if (!ok) break;
+          if (elect_one()) {
+            tc::mma_commit(&bar.a);
+            tc::mma_commit(&bar.ox_empty);
+            tc::mma_commit(&bar.ex_empty);
+          }
+          __syncwarp();
           ok = wait(&bar.nm, ph);
           if (!ok) break;
           tc::fence_after_sync();
           if (elect_one()) {
-#pragma unroll 1
+#pragma unroll
             for (int s = 0; s < 4; ++s) {
-              tc::mma_bf16(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
-              tc::mma_bf16(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
-              tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
-              tc::mma_bf16(tb + cF + 64, dKn + nstep(s), dM + nstep(s), idMM, true);
-              tc::mma_bf16(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
+              mma_ss(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
+              mma_ss(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
+              mma_ss(tb + cF + 64, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
+              mma_ss(tb + cF + 64, dKn + nstep(s), dM + nstep(s), idMM, true);
+              mma_ss(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
             }
             tc::mma_commit(&bar.a45);
             if (h == hpg - 1) tc::mma_commit(&bar.qk_empty);
@@ -367,17 +367,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             c[k] = (sm.c[0][j] + sm.c[1][j]) + (sm.c[2][j] + sm.c[3][j]);  // w_j k_j . a3_j
           }
           const float b0 = gate[kGateBeta + 2 * lane], b1 = gate[kGateBeta + 2 * lane + 1];
+          // the rows' sums over their first 32 columns, which R lacks past them
+          const float s0 = sm.base[2 * lane] + sm.base[64 + 2 * lane], s1 = sm.base[2 * lane + 1] + sm.base[65 + 2 * lane];
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(&bar.fin);
             mbar_arrive(&bar.g_empty[hc & 1]);
           }
-          float pre = b0 * c[0] + b1 * c[1], suf = r[0] + r[1];  // sums up to and from this lane's tokens
+          float pre = b0 * c[0] + b1 * c[1], suf = r[0] + r[1], left = s0 + s1;  // sums up to and from this lane's tokens
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const float a = __shfl_up_sync(0xffffffffu, pre, o), b = __shfl_down_sync(0xffffffffu, suf, o);
+            const float e = __shfl_down_sync(0xffffffffu, left, o);
             if (lane >= o) pre += a;
-            if (lane + o < 32) suf += b;
+            if (lane + o < 32) suf += b, left += e;
+          }
+          if (lane >= 16) {
+            R[0] += left;
+            R[1] += left - s0;
           }
           const float before = __shfl_up_sync(0xffffffffu, pre, 1);
           const float after = __shfl_down_sync(0xffffffffu, suf, 1);
@@ -510,87 +517,80 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait(&bar.g_full[hc & 1], (hc / 2) & 1) && wait(&bar.f, ph);
         if (!ok) break;
         tc::fence_after_sync();
-        {  // rows: f and qk (lanes 0-63), F' and kk (64-127); columns c0 ..
+        {  // rows: f and qk (lanes 0-63), F' and kk (64-127); columns c0 .., 16 at a time
           const int i = row & 63;
           const bool second = quarter >= 2;
-          float x[32];
-          {
-            float a[32];
-            tmem_ld32(tb + tl + cF + c0, x);
-            tmem_ld32(tb + tl + cF + 64 + c0, a);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] += a[k];
-            const float own = second ? 1.f : 0.f;  // (the upper rows of the third part are E E^t)
-            tmem_ld32(tb + tl + cF + 128 + c0, a);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = fmaf(own, a[k], x[k]);
-          }
-          const float bi = gate[kGateB + i];
-          const float sc = second ? -1.f : p.scale;
-          const int lim = (second ? i - 1 : i) - c0;  // last of these columns in the row
+          const float own = second ? 1.f : 0.f;  // (the upper rows of the third part are E E^t)
+          const float bi = gate[kGateB + i], sc = second ? -1.f : p.scale;
           const uint32_t wide = __float_as_uint(gate[kGateWide]);
-#pragma unroll
+          unsigned char* tile = smem + lay.nm + (second ? kTile : 0);
+          ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
+          if (!ok) break;
+          float run = 0.f;
+#pragma unroll 1
           for (int g = 0; g < 2; ++g) {
-            float f[16];
-            if ((wide >> (8 * (2 * hf + g))) & 1u) {
+            const int cg = c0 + 16 * g, lim = (second ? i - 1 : i) - cg;  // last of these columns in the row
+            float x[16];
+            {
+              float a[16], b[16];
+              tc::tmem_ld16(tb + tl + cF + cg, x);
+              tc::tmem_ld16(tb + tl + cF + 64 + cg, a);
+              tc::tmem_ld16(tb + tl + cF + 128 + cg, b);
+              tc::tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 16; ++k) f[k] = sc * __expf(bi - gate[kGateB + c0 + 16 * g + k]);
+              for (int k = 0; k < 16; ++k) x[k] = fmaf(own, b[k], x[k] + a[k]);
+            }
+            if ((wide >> (cg / 2)) & 1u) {  // bit 8 of a 16-token group
+#pragma unroll
+              for (int k = 0; k < 16; ++k) x[k] *= sc * __expf(bi - gate[kGateB + cg + k]);
             } else {
-              const float rf = sc * __expf(bi - gate[kGateB + c0 + 16 * g]);
+              const float rf = sc * __expf(bi - gate[kGateB + cg]);
 #pragma unroll
               for (int k = 0; k < 16; k += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(gate + kGateKey + c0 + 16 * g + k);
-                f[k] = rf * k4.x, f[k + 1] = rf * k4.y, f[k + 2] = rf * k4.z, f[k + 3] = rf * k4.w;
+                const float4 k4 = *reinterpret_cast<const float4*>(gate + kGateKey + cg + k);
+                x[k] *= rf * k4.x, x[k + 1] *= rf * k4.y, x[k + 2] *= rf * k4.z, x[k + 3] *= rf * k4.w;
+              }
+            }
+            float R[16];  // beta y later; first beta x, which is N or M
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              const float4 b4 = *reinterpret_cast<const float4*>(gate + kGateBeta + cg + k);
+              const float be[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                x[k + m] = k + m <= lim ? x[k + m] : 0.f;
+                R[k + m] = be[m] * x[k + m];
               }
             }
 #pragma unroll
-            for (int k = 0; k < 16; ++k) x[16 * g + k] = 16 * g + k <= lim ? f[k] * x[16 * g + k] : 0.f;
-          }
-          ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
-          if (!ok) break;
-          unsigned char* tile = smem + lay.nm + (second ? kTile : 0);
+            for (int k = 0; k < 2; ++k) {
+              uint32_t o[4], l[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t o[4], l[4];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const float2 be = *reinterpret_cast<const float2*>(gate + kGateBeta + c0 + 8 * k + 2 * m);
-              split2(f2_mul(be, make_float2(x[8 * k + 2 * m], x[8 * k + 2 * m + 1])), o[m], l[m]);
+              for (int m = 0; m < 4; ++m) split2(make_float2(R[8 * k + 2 * m], R[8 * k + 2 * m + 1]), o[m], l[m]);
+              const uint32_t to = tc::chunk_off(i, cg / 8 + k);
+              *reinterpret_cast<uint4*>(tile + to) = make_uint4(o[0], o[1], o[2], o[3]);
+              if (!second) *reinterpret_cast<uint4*>(smem + lay.out + to) = make_uint4(l[0], l[1], l[2], l[3]);
             }
-            const uint32_t to = tc::chunk_off(i, 4 * hf + k);
-            *reinterpret_cast<uint4*>(tile + to) = make_uint4(o[0], o[1], o[2], o[3]);
-            if (!second) *reinterpret_cast<uint4*>(smem + lay.out + to) = make_uint4(l[0], l[1], l[2], l[3]);
-          }
-          fence_proxy_async_smem();
-          float prod[32];
-          tmem_ld32(tb + tl + cKQ + c0, prod);
-          tc::tmem_wait_ld();
-          arrive(&bar.nm);
-          // y, and the prefixes of beta y along the row that reach column t <= i
-          float R[32], run = 0.f;
+            // y, and the prefixes of beta y along the row that reach column t <= i
+            float prod[16];
+            tc::tmem_ld16(tb + tl + cKQ + cg, prod);
+            tc::tmem_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 b4 = *reinterpret_cast<const float4*>(gate + kGateBeta + c0 + k);
-            const float be[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              x[k + m] *= prod[k + m];
-              R[k + m] = run;
-              run = fmaf(be[m], x[k + m], run);
+            for (int k = 0; k < 16; ++k) {
+              x[k] *= prod[k];
+              const float by = R[k] * prod[k];
+              R[k] = k <= i - cg ? run : 0.f;
+              run += by;
+            }
+            const float y = column_sums(x, lane), Rs = column_sums(R, lane);
+            if ((lane & 1) == 0) {
+              sm.y[quarter][cg + (lane >> 1)] = y;
+              sm.R[quarter][cg + (lane >> 1)] = Rs;
             }
           }
           if (hf == 0) sm.base[row] = run;
-          const float y = column_sums(x, lane);
-          ok = meet(&bar.epi_sync);
-          if (!ok) break;
-          const float base = hf == 0 ? 0.f : sm.base[row];
-#pragma unroll
-          for (int k = 0; k < 32; ++k) R[k] = k <= i - c0 ? R[k] + base : 0.f;
-          const float Rs = column_sums(R, lane);
-          sm.y[quarter][c0 + lane] = y;
-          sm.R[quarter][c0 + lane] = Rs;
+          fence_proxy_async_smem();
+          arrive(&bar.nm);
         }
         // state columns as lanes: a1, a2, a3
         ok = wait(&bar.a, ph);
@@ -603,60 +603,55 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto elem = [&](const unsigned char* tile, int k) {
             return to_f32(*reinterpret_cast<const __nv_bfloat16*>(tile + k * 128 + (col ^ ((k & 7) << 4))));
           };
-          float s[32], kv[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) kv[k] = elem(tq + kTile, k);
-          {
-            float a[32];
-            tmem_ld32(tb + tl + cA + c0, a);
+          for (int g = 0; g < 2; ++g) {
+            const int cg = c0 + 16 * g;
+            float s[16], kv[16], a[16], b[16];
+            tc::tmem_ld16(tb + tl + cA + cg, a);
+            tc::tmem_ld16(tb + tl + cA + 64 + cg, b);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) kv[k] = elem(tq + kTile, 16 * g + k);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + c0 + k);
+            for (int k = 0; k < 16; k += 2) {
+              const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + cg + k);
               const float v0 = -p.scale * e.x * a[k], v1 = -p.scale * e.y * a[k + 1];
-              dq[k] += v0;
-              dq[k + 1] += v1;
-              s[k] = v0 * elem(tq, k);
-              s[k + 1] = v1 * elem(tq, k + 1);
+              const float u0 = e.x * b[k], u1 = e.y * b[k + 1];
+              dq[16 * g + k] += v0;
+              dq[16 * g + k + 1] += v1;
+              dk[16 * g + k] += u0;
+              dk[16 * g + k + 1] += u1;
+              s[k] = fmaf(u0, kv[k], v0 * elem(tq, 16 * g + k));
+              s[k + 1] = fmaf(u1, kv[k + 1], v1 * elem(tq, 16 * g + k + 1));
             }
-            tmem_ld32(tb + tl + cA + 64 + c0, a);
+            if (K == 64 && !klive) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) s[k] = 0.f;
+            }
+            const float r = column_sums(s, lane);
+            tc::tmem_ld16(tb + tl + cA3 + cg, a);
+            tc::tmem_ld16(tb + tl + cA3 + 64 + cg, b);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + c0 + k);
-              const float v0 = e.x * a[k], v1 = e.y * a[k + 1];
-              dk[k] += v0;
-              dk[k + 1] += v1;
-              s[k] = fmaf(v0, kv[k], s[k]);
-              s[k + 1] = fmaf(v1, kv[k + 1], s[k + 1]);
-            }
-          }
-          if (K == 64 && !klive) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[k] = 0.f;
-          }
-          sm.r[quarter][c0 + lane] = column_sums(s, lane);
-          {
-            float a[32], b[32];
-            tmem_ld32(tb + tl + cA3 + c0, a);
-            tmem_ld32(tb + tl + cA3 + 64 + c0, b);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float2 bw = *reinterpret_cast<const float2*>(gate + kGateW + c0 + k);
-              const float2 wt = *reinterpret_cast<const float2*>(gate + kGateTail + c0 + k);
+            for (int k = 0; k < 16; k += 2) {
+              const float2 bw = *reinterpret_cast<const float2*>(gate + kGateW + cg + k);
+              const float2 wt = *reinterpret_cast<const float2*>(gate + kGateTail + cg + k);
               const float v0 = a[k] + b[k], v1 = a[k + 1] + b[k + 1];
-              dk[k] = fmaf(bw.x, v0, dk[k]);
-              dk[k + 1] = fmaf(bw.y, v1, dk[k + 1]);
+              dk[16 * g + k] = fmaf(bw.x, v0, dk[16 * g + k]);
+              dk[16 * g + k + 1] = fmaf(bw.y, v1, dk[16 * g + k + 1]);
               s[k] = wt.x * v0 * kv[k];
               s[k + 1] = wt.y * v1 * kv[k + 1];
             }
-          }
-          if (K == 64 && !klive) {
+            if (K == 64 && !klive) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) s[k] = 0.f;
+              for (int k = 0; k < 16; ++k) s[k] = 0.f;
+            }
+            const float c = column_sums(s, lane);
+            if ((lane & 1) == 0) {
+              sm.r[quarter][cg + (lane >> 1)] = r;
+              sm.c[quarter][cg + (lane >> 1)] = c;
+            }
           }
-          sm.c[quarter][c0 + lane] = column_sums(s, lane);
         }
         __syncwarp();
         if (lane == 0) {
@@ -667,14 +662,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc::fence_after_sync();
         {
-          float a[32], b[32];
-          tmem_ld32(tb + tl + cF + c0, a);
-          tmem_ld32(tb + tl + cF + 64 + c0, b);
-          tc::tmem_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            dq[k] += a[k];
-            dk[k] += b[k];
+          for (int g = 0; g < 2; ++g) {
+            float a[16], b[16];
+            tc::tmem_ld16(tb + tl + cF + c0 + 16 * g, a);
+            tc::tmem_ld16(tb + tl + cF + 64 + c0 + 16 * g, b);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              dq[16 * g + k] += a[k];
+              dk[16 * g + k] += b[k];
+            }
           }
         }
         arrive(&bar.free);
