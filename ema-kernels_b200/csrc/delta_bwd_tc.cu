@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   auto wait1 = [&](uint64_t* b, uint32_t parity) { return chain_wait(b, parity, status, fail); };
-  auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait1(b, parity)) != 0; };
+  auto wait = [&](uint64_t* b, uint32_t parity) { return chain_wait_warp(b, parity, status, fail); };
   auto chunk = [&](int r) { return nc - 1 - r; };  // of step r
 
   if (warp >= kMma) {

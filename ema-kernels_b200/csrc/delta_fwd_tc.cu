@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // a wait that runs out marks the block as failed; every role then leaves its loop at the next wait, warps as a whole
   auto wait1 = [&](uint64_t* b, uint32_t parity) { return chain_wait(b, parity, status, fail); };
-  auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait1(b, parity)) != 0; };
+  auto wait = [&](uint64_t* b, uint32_t parity) { return chain_wait_warp(b, parity, status, fail); };
 
   if (warp >= kMma) {
     set_regs_down<kRegCtl>();

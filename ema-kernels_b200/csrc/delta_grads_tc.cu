@@ -17,7 +17,7 @@
 //
 // One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  S0, dS1, E
 // and dX come as fp32 images; warps 8-11 take them through registers, sum <dS1, S0> on the way and stage the pieces, S0 and
-// dS1 in steps of 16 value channels (one MMA step) through a ring of two.  Bound: the images' bytes (S0 and dS1 are 2 x 64
+// dS1 in steps of 16 value channels (one MMA step) through a ring of four.  Bound: the images' bytes (S0 and dS1 are 2 x 64
 // KB a chunk and head at 128 x 128), and near it the tensor pipe (about 7500 cycles a head) and the epilogues.  Roles: warps
 // 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 staging, warp 12 the MMAs, warp 13 the loads of Q, K, dO
 // and dv, warp 14 dg and dbeta from the epilogues' sums.  The long loops are kept rolled where they can be: at twice the
@@ -39,7 +39,7 @@ constexpr int kMma = 12, kLoad = 13, kGates = 14;  // (15 only fills its warpgro
 constexpr int kThreads = 16 * 32;
 constexpr int kRegEpi = 152, kRegAux = 128, kRegCtl = 80;
 static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128 && kRegAux >= 128 && kRegCtl <= 128, "register split");
-constexpr int kRing = 2;
+constexpr int kRing = 4;
 constexpr int kReg = 128 * 128;  // two 64-row tiles of 64 columns, one over the other
 
 // tensor-memory columns
@@ -50,7 +50,7 @@ constexpr uint32_t cA3 = 384;   // a3 of E hi and lo, of E mid
 
 struct Bars {
   uint64_t qk_full, qk_empty, ox_full, ox_empty, ex_full, ex_empty;
-  uint64_t s_full[kRing], s_empty[kRing];  // S0 and dS1, 16 value channels each
+  uint64_t s_full[kRing], s_empty[kRing];  // 16 value channels of S0 (even slots) or dS1 (odd)
   uint64_t g_full[2], g_empty[2];
   uint64_t f, a, a45;          // MMA groups done
   uint64_t nm, free;           // N, M written; all accumulators read
@@ -68,21 +68,18 @@ struct Small {
   Bars bar;
 };
 
-// Offsets from the 1024-byte aligned base, by the padded channel count.
-template <int K>
+// Offsets from the 1024-byte aligned base.
+template <int K, int VP>
 struct Layout {
   static constexpr int kPiece = 16 * K * 2;     // 16 state rows of one piece: a 2 KB tile per 64 columns
-  static constexpr int kStep = 6 * kPiece;      // S0 hi, mid, lo, dS1 hi, mid, lo
-  int ox, ex, ring, nm, out, small;
-  __host__ __device__ explicit Layout(int VP) {
-    ox = (K / 64) * kReg;                       // after [Q; K]
-    ex = ox + (VP / 64) * kReg;                 // E hi, mid, lo, dX lo
-    ring = ex + 4 * VP * 128;
-    nm = ring + kRing * kStep;                  // N, M
-    out = nm + 2 * kTile;                       // N lo; 32 rows of dq or dk on their way out
-    small = out + kTile;                        // (32 x dstate bf16 fit it)
-  }
-  __host__ __device__ int bytes() const { return small + static_cast<int>(sizeof(Small)); }
+  static constexpr int kStep = 3 * kPiece;      // hi, mid, lo of S0 or dS1
+  static constexpr int ox = (K / 64) * kReg;             // after [Q; K]
+  static constexpr int ex = ox + (VP / 64) * kReg;       // E hi, mid, lo, dX lo
+  static constexpr int ring = ex + 4 * VP * 128;
+  static constexpr int nm = ring + kRing * kStep;        // N, M
+  static constexpr int out = nm + 2 * kTile;             // N lo; 32 rows of dq or dk on their way out
+  static constexpr int small = out + kTile;              // (32 x dstate bf16 fit it)
+  static constexpr int bytes = small + static_cast<int>(sizeof(Small));
 };
 
 // Columns 8 chunk .. 8 chunk + 7 of a row of an fp32 image.
@@ -122,15 +119,15 @@ __device__ __forceinline__ float column_sums(float (&x)[16], int lane) {
   return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 1);
 }
 
-template <int K>
+template <int K, int VP>
 __global__ void __launch_bounds__(kThreads, 1)
     grads_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq,
                     const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap mdv, const Params p,
                     const TcBuffers w, uint32_t* status) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  const int VP = pad_channels(p.V), img = VP * 128, steps = VP / 16;
-  const Layout<K> lay(VP);
-  Small& sm = *reinterpret_cast<Small*>(smem + lay.small);
+  using Lay = Layout<K, VP>;
+  constexpr int img = VP * 128, steps = VP / 16;
+  Small& sm = *reinterpret_cast<Small*>(smem + Lay::small);
   Bars& bar = sm.bar;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hpg = p.H / p.G;
@@ -139,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     uint64_t* one[] = {&bar.qk_full, &bar.ox_full, &bar.ox_empty, &bar.ex_empty, &bar.s_empty[0], &bar.s_empty[1],
-                       &bar.g_full[0], &bar.g_full[1], &bar.f, &bar.a, &bar.a45, &bar.fin, &bar.drain};
+                       &bar.s_empty[2], &bar.s_empty[3], &bar.g_full[0], &bar.g_full[1], &bar.f, &bar.a, &bar.a45, &bar.fin, &bar.drain};
     for (uint64_t* b : one) mbar_init(b, 1);
     mbar_init(&bar.qk_empty, 1 + kEpi);
     mbar_init(&bar.ex_full, kAux);
@@ -165,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   auto wait1 = [&](uint64_t* b, uint32_t parity) { return chain_wait(b, parity, status, fail); };
-  auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait1(b, parity)) != 0; };
+  auto wait = [&](uint64_t* b, uint32_t parity) { return chain_wait_warp(b, parity, status, fail); };
   uint32_t meetings = 0;
   auto meet = [&](uint64_t* b) {
     __syncwarp();
@@ -203,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (hc > 0 && !(ok = wait1(&bar.ox_empty, last))) break;
           mbar_arrive_expect_tx(&bar.ox_full, (VP / 64) * kReg);
           for (int i = 0; i < VP / 64; ++i) {
-            tma_load_4d(smem + lay.ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
-            tma_load_4d(smem + lay.ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
+            tma_load_4d(smem + Lay::ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
+            tma_load_4d(smem + Lay::ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
           }
         }
       }
@@ -229,15 +226,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t sreg = K == 128 ? 2048u : 0u, qreg = K == 128 ? kReg : 0u;
       const uint32_t dQK = desc_lo(sb, 16), dK = desc_lo(sb + kTile, 16);
       const uint32_t dQn = desc_lo(sb, qreg), dKn = desc_lo(sb + kTile, qreg);
-      const uint32_t dOX = desc_lo(sb + lay.ox, 16);
-      const uint32_t dE = desc_lo(sb + lay.ex, img);            // [E hi | E mid]
-      const uint32_t dEm = desc_lo(sb + lay.ex + img, img);     // E mid
-      const uint32_t dEl = desc_lo(sb + lay.ex + 2 * img, img); // E lo
-      const uint32_t dEX = desc_lo(sb + lay.ex, 3 * img);       // [E hi | dX lo]
-      const uint32_t dXl = desc_lo(sb + lay.ex + 3 * img, img);
-      const uint32_t dRing = desc_lo(sb + lay.ring, sreg);
-      const uint32_t dN = desc_lo(sb + lay.nm, 16), dM = desc_lo(sb + lay.nm + kTile, 16);
-      const uint32_t dNl = desc_lo(sb + lay.out, 16);
+      const uint32_t dOX = desc_lo(sb + Lay::ox, 16);
+      const uint32_t dE = desc_lo(sb + Lay::ex, img);            // [E hi | E mid]
+      const uint32_t dEm = desc_lo(sb + Lay::ex + img, img);     // E mid
+      const uint32_t dEl = desc_lo(sb + Lay::ex + 2 * img, img); // E lo
+      const uint32_t dEX = desc_lo(sb + Lay::ex, 3 * img);       // [E hi | dX lo]
+      const uint32_t dXl = desc_lo(sb + Lay::ex + 3 * img, img);
+      const uint32_t dRing = desc_lo(sb + Lay::ring, sreg);
+      const uint32_t dN = desc_lo(sb + Lay::nm, 16), dM = desc_lo(sb + Lay::nm + kTile, 16);
+      const uint32_t dNl = desc_lo(sb + Lay::out, 16);
       int n, tok, task = 0, hc = 0, rc = 0;
       Seq q;
       bool ok = true;
@@ -260,8 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait(&bar.ox_full, ph) && wait(&bar.ex_full, ph);
           if (!ok) break;
           if (cut) {
-            zero_rows(smem + lay.ox, VP / 64, kReg, have);
-            zero_rows(smem + lay.ox + kTile, VP / 64, kReg, have);
+            zero_rows(smem + Lay::ox, VP / 64, kReg, have);
+            zero_rows(smem + Lay::ox + kTile, VP / 64, kReg, have);
             fence_proxy_async_smem();
             __syncwarp();
           }
@@ -275,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll 1
             for (int s4 = 0; s4 < steps / 4; ++s4) {  // 64 value channels
-              const uint32_t ox = dOX + s4 * (kReg >> 4), vo = static_cast<uint32_t>(s4 * 512);
+              const uint32_t ox = dOX + s4 * (kReg >> 4), vo = s4 * 512;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const bool more = s4 > 0 || i > 0;
@@ -289,27 +286,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
 #pragma unroll 1
-          for (int s4 = 0; ok && s4 < steps / 4; ++s4) {
-            const uint32_t ox = dOX + s4 * (kReg >> 4), vo = static_cast<uint32_t>(s4 * 512);
+          for (int s2 = 0; ok && s2 < steps / 2; ++s2, ++rc) {  // the ring once around: two steps, S0 and dS1 of each
+            const uint32_t ox = dOX + (s2 >> 1) * (kReg >> 4) + (s2 & 1) * 4, vo = s2 * 256;
 #pragma unroll
-            for (int i = 0; i < 4; ++i, ++rc) {  // (steps is a multiple of the ring: step i uses slot i % kRing)
-              const int st = i % kRing;
-              ok = ok && wait(&bar.s_full[st], (rc / kRing) & 1);
+            for (int i = 0; i < 2; ++i) {
+              constexpr uint32_t pc = Lay::kPiece >> 4, slot16 = Lay::kStep >> 4;
+              const uint32_t dS = dRing + 2 * i * slot16, dD = dS + slot16;
+              const bool more = s2 > 0 || i > 0;
+              ok = ok && wait(&bar.s_full[2 * i], rc & 1);
               if (!ok) break;
-              constexpr uint32_t pc = Layout<K>::kPiece >> 4;
-              const uint32_t dS = dRing + st * (Layout<K>::kStep >> 4), dD = dS + 3 * pc;
               if (elect_one()) {
-                const bool more = s4 > 0 || i > 0;
                 mma_ss(tb + cA, dS, ox + 2 * i, idA, more);
                 mma_ss(tb + cA, dS + pc, ox + 2 * i, idA, true);
                 mma_ss(tb + cA, dS + 2 * pc, ox + 2 * i, idA, true);
                 mma_ss(tb + cA + 64, dS, dXl + vo + 128 * i, idMM, true);
                 mma_ss(tb + cA + 64, dS + pc, dXl + vo + 128 * i, idMM, true);
+                tc::mma_commit(&bar.s_empty[2 * i]);
+              }
+              __syncwarp();
+              ok = wait(&bar.s_full[2 * i + 1], rc & 1);
+              if (!ok) break;
+              if (elect_one()) {
                 mma_ss(tb + cA3, dD, dE + vo + 128 * i, idMM128, more);
                 mma_ss(tb + cA3, dD + pc, dE + vo + 128 * i, idMM128, true);
                 mma_ss(tb + cA3, dD, dEl + vo + 128 * i, idMM, true);
                 mma_ss(tb + cA3, dD + 2 * pc, dE + vo + 128 * i, idMM, true);
-                tc::mma_commit(&bar.s_empty[st]);
+                tc::mma_commit(&bar.s_empty[2 * i + 1]);
               }
               __syncwarp();
             }
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = c0; c < 8; c += 2 * cs) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            unsigned char* to = smem + lay.ex + tc::chunk_off(row, c + k * cs);
+            unsigned char* to = smem + Lay::ex + tc::chunk_off(row, c + k * cs);
             stage_row8(to, img, e[k]);
             stage_lo8(to + 3 * img, x[k]);  // dX hi is dv
           }
@@ -459,23 +461,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         publish(&bar.ex_full);
         fetch(1, 1);
 #pragma unroll 1
-        for (int s2 = 0; ok && s2 < steps; s2 += 2) {
+        for (int s2 = 0; ok && s2 < steps; s2 += 2, ++rc) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u, ++rc) {
-            const int st = rc % kRing;
-            ok = ok && (rc < kRing || wait(&bar.s_empty[st], (rc / kRing - 1) & 1));
+          for (int u = 0; u < 2; ++u) {
+            ok = ok && (rc == 0 || wait(&bar.s_empty[2 * u], (rc - 1) & 1));
             if (!ok) break;
-            unsigned char* base = smem + lay.ring + st * Layout<K>::kStep;
+            unsigned char* base = smem + Lay::ring + 2 * u * Lay::kStep;
 #pragma unroll
             for (int k = 0; k < kItems; ++k) {
               const int i = at + k * kAux * 32, r = i & 15, c = i >> 4;
 #pragma unroll
               for (int m = 0; m < 4; ++m) acc = f2_fma(s0[u][k][m], d1[u][k][m], acc);
-              unsigned char* to = base + (c >> 3) * 2048 + tc::chunk_off(r, c & 7);
-              stage_row8(to, Layout<K>::kPiece, s0[u][k]);
-              stage_row8(to + 3 * Layout<K>::kPiece, Layout<K>::kPiece, d1[u][k]);
+              stage_row8(base + (c >> 3) * 2048 + tc::chunk_off(r, c & 7), Lay::kPiece, s0[u][k]);
             }
-            publish(&bar.s_full[st]);
+            publish(&bar.s_full[2 * u]);
+            ok = rc == 0 || wait(&bar.s_empty[2 * u + 1], (rc - 1) & 1);
+            if (!ok) break;
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+              const int i = at + k * kAux * 32, r = i & 15, c = i >> 4;
+              stage_row8(base + Lay::kStep + (c >> 3) * 2048 + tc::chunk_off(r, c & 7), Lay::kPiece, d1[u][k]);
+            }
+            publish(&bar.s_full[2 * u + 1]);
             if (s2 + 2 < steps) fetch(s2 + 2 + u, u);
           }
         }
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float own = second ? 1.f : 0.f;  // (the upper rows of the third part are E E^t)
           const float bi = gate[kGateB + i], sc = second ? -1.f : p.scale;
           const uint32_t wide = __float_as_uint(gate[kGateWide]);
-          unsigned char* tile = smem + lay.nm + (second ? kTile : 0);
+          unsigned char* tile = smem + Lay::nm + (second ? kTile : 0);
           ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
           if (!ok) break;
           float run = 0.f;
@@ -569,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int m = 0; m < 4; ++m) split2(make_float2(R[8 * k + 2 * m], R[8 * k + 2 * m + 1]), o[m], l[m]);
               const uint32_t to = tc::chunk_off(i, cg / 8 + k);
               *reinterpret_cast<uint4*>(tile + to) = make_uint4(o[0], o[1], o[2], o[3]);
-              if (!second) *reinterpret_cast<uint4*>(smem + lay.out + to) = make_uint4(l[0], l[1], l[2], l[3]);
+              if (!second) *reinterpret_cast<uint4*>(smem + Lay::out + to) = make_uint4(l[0], l[1], l[2], l[3]);
             }
             // y, and the prefixes of beta y along the row that reach column t <= i
             float prod[16];
@@ -693,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = meet(&bar.epi_sync);  // the tile's last pieces have been read
         if (!ok) break;
         if (klive && hf == half) {
-          uint16_t* so = reinterpret_cast<uint16_t*>(smem + lay.out) + row;
+          uint16_t* so = reinterpret_cast<uint16_t*>(smem + Lay::out) + row;
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const uint32_t v = which == 0 ? qo[k] : ko[k];
@@ -709,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const View& v = which == 0 ? p.vdq : p.vdk;
         for (int tk = tid / kPieces; tk < 32 && 32 * half + tk < have; tk += kRows)
           __stcs(reinterpret_cast<uint4*>(row_of<__nv_bfloat16>(out, v, q.b, q.t0 + tok + 32 * half + tk, gr)) + pc,
-                 *reinterpret_cast<const uint4*>(smem + lay.out + (tk * kPieces + pc) * 16));
+                 *reinterpret_cast<const uint4*>(smem + Lay::out + (tk * kPieces + pc) * 16));
       }
       ok = ok && meet(&bar.epi_sync);  // N lo of the next head goes where they were
     }
@@ -722,19 +729,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int K>
+template <int K, int VP>
 cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mq, const CUtensorMap& mo, const CUtensorMap& mdv,
                    const Params& p, const TcBuffers& w, uint32_t* status, cudaStream_t st) {
   static unsigned long long mask = 0;
-  const int most = Layout<K>(128).bytes() > Layout<K>(64).bytes() ? Layout<K>(128).bytes() : Layout<K>(64).bytes();
-  cudaError_t e = static_cast<cudaError_t>(
-      ensure_smem_attr(reinterpret_cast<const void*>(grads_tc_kernel<K>), most, &mask));
+  constexpr int bytes = Layout<K, VP>::bytes;
+  static_assert(bytes <= kMaxDynSmem, "shared memory");
+  const cudaError_t e = static_cast<cudaError_t>(
+      ensure_smem_attr(reinterpret_cast<const void*>(grads_tc_kernel<K, VP>), bytes, &mask));
   if (e != cudaSuccess) return e;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const long long tasks = static_cast<long long>(p.slots) * p.G;
-  grads_tc_kernel<K><<<static_cast<unsigned>(tasks < sms ? tasks : sms), kThreads, Layout<K>(pad_channels(p.V)).bytes(),
-                       st>>>(mk, mq, mo, mdv, p, w, status);
+  grads_tc_kernel<K, VP><<<static_cast<unsigned>(tasks < sms ? tasks : sms), kThreads, bytes, st>>>(mk, mq, mo, mdv, p, w,
+                                                                                                 status);
   return cudaGetLastError();
 }
 
@@ -743,7 +751,10 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mq, const CUtensorM
 cudaError_t tc_grads(const CUtensorMap& mk, const CUtensorMap& mq, const CUtensorMap& mo, const CUtensorMap& mdv,
                      const Params& p, const TcBuffers& w, uint32_t* status, cudaStream_t st) {
   if (p.slots == 0) return cudaSuccess;
-  return p.K == 64 ? launch<64>(mk, mq, mo, mdv, p, w, status, st) : launch<128>(mk, mq, mo, mdv, p, w, status, st);
+  const bool wide = pad_channels(p.V) == 128;
+  if (p.K == 64)
+    return wide ? launch<64, 128>(mk, mq, mo, mdv, p, w, status, st) : launch<64, 64>(mk, mq, mo, mdv, p, w, status, st);
+  return wide ? launch<128, 128>(mk, mq, mo, mdv, p, w, status, st) : launch<128, 64>(mk, mq, mo, mdv, p, w, status, st);
 }
 
 }  // namespace delta

@@ -117,19 +117,29 @@ __device__ __forceinline__ void set_regs_down() {
 }
 
 // Bounded wait of the chain's roles: no sleep between the polls (a poll suspends the thread in hardware for a
-// while by itself), since every nanosecond after the phase completes is on the chain, and few instructions: the
-// kernels' loops are long and instruction fetches from beyond the caches cost more than the waits.
+// while by itself), since every nanosecond after the phase completes is on the chain.  The first poll stands alone: a phase
+// that is complete already (most are) costs that and a vote, no clock and no look at the block's failure word.
 constexpr long long kWaitLimitCycles = 2000000000ll;  // about a second
-__device__ __forceinline__ bool chain_wait(uint64_t* bar, uint32_t phase, uint32_t* status, volatile uint32_t* fail) {
+__device__ __forceinline__ bool chain_wait_slow(uint64_t* bar, uint32_t phase, uint32_t* status, volatile uint32_t* fail) {
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, phase)) {
+    if (*fail != 0u) return false;
     if (clock64() - t0 > kWaitLimitCycles) {
       atomicOr(status, kStatusTmaTimeout);
       *fail = 1u;
-      break;
+      return false;
     }
   }
-  return *fail == 0u;
+  return true;
+}
+// By one thread.
+__device__ __forceinline__ bool chain_wait(uint64_t* bar, uint32_t phase, uint32_t* status, volatile uint32_t* fail) {
+  return mbar_try_wait(bar, phase) || chain_wait_slow(bar, phase, status, fail);
+}
+// By a whole warp, with one answer.
+__device__ __forceinline__ bool chain_wait_warp(uint64_t* bar, uint32_t phase, uint32_t* status, volatile uint32_t* fail) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
+  return __all_sync(0xffffffffu, chain_wait_slow(bar, phase, status, fail)) != 0;
 }
 
 // Zero rows [from, 64) of `regions` 64-row regions `stride` bytes apart (one warp).
