@@ -11,10 +11,14 @@
 // for E and U P^t; w U, whose rounding stays in the state, is three pieces.  (o = scale exp(b) S Q^t + U P^t ends in bf16, but where keys repeat its two terms
 // cancel: hi parts alone left it 1e-2 off there.)
 //
-// Bound: the chain's latency.  A chunk is three dependent MMA groups (about 1000, 640 and 770 cycles at dstate
-// 128) with an epilogue after each (600, 750 and 980); the products for o run in their shadow.  Roles: warps 0-7 the chain's epilogues
+// Bound: the chain's latency, 6100 cycles a chunk at dstate 128 (16384 tokens of 32 heads of 128: 850 us; 40 sequences, 8111
+// tokens of 16 heads: 118): three dependent MMA groups (about 1000, 640 and 950 cycles) with an epilogue after each (600,
+// 750 and 980) and the hand-overs between them; the products for o run in their shadow.  A training forward with a block on
+// most SMs is near its bytes instead: it writes S, E and o, 128 KB a chunk and head (4 x 4096 x 32: 310 us, 3.6 TB/s of writes
+// and 0.9 of reads).  Roles: warps 0-7 the chain's epilogues
 // (warp w: lanes 32 (w % 4), half w / 4 of the columns; the fp32 state lives in their registers), warps 8-11 the
-// output, warp 12 issues the MMAs, warp 13 the loads (TMA for K, Q, V; bulk copies for the images), two stages deep.
+// output, warp 12 issues the MMAs, warp 13 the loads (TMA for K, Q, V; bulk copies for the images), two stages deep, warp
+// 14 E's copies to memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -29,12 +33,13 @@ namespace {
 
 constexpr int kEpi = 8;                      // epilogue warps
 constexpr int kOut = 4;                      // output warps
-constexpr int kMma = 12, kLoad = 13;         // (14 and 15 only fill their warpgroup)
+constexpr int kMma = 12, kLoad = 13, kStore = 14;  // (15 only fills its warpgroup)
 constexpr int kThreads = 16 * 32;
 // registers a thread, by warpgroup: 2 epilogue, output, MMA and loads; 4 x 128 at launch
 constexpr int kRegEpi = 160, kRegOut = 120, kRegCtl = 72;
 static_assert(2 * kRegEpi + kRegOut + kRegCtl == 4 * 128, "register split");
 constexpr int kStages = 2;
+constexpr int kKeep = 3 * 2 * kTile;
 constexpr int kReg = 128 * 128;              // 64 query rows, then 64 key rows of 64 columns
 
 // tensor-memory columns.  An MMA step with its left operand in tensor memory takes about 32 + N / 2 cycles here, so what
@@ -51,6 +56,7 @@ struct Bars {
   uint64_t ks, qs, e, ds, pu;  // MMA groups done
   uint64_t s, x, wu, u;    // epilogues done: state, X, w U and U ready
   uint64_t q, o;           // Q S, U P read
+  uint64_t ek, ekfree;     // E's pieces staged, and on their way to memory
   uint64_t out_sync;       // meeting of the output warps (bounded, unlike a barrier instruction)
   uint64_t drain;          // MMAs still in flight after a failed wait
   uint32_t taddr, fail;
@@ -76,7 +82,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const __grid_constant__ CUtensorMap mv, const Params p, const TcBuffers w, uint32_t* status) {
   using St = Stage<K>;
   extern __shared__ __align__(1024) unsigned char smem[];
-  Bars& bar = *reinterpret_cast<Bars*>(smem + kStages * St::kBytes);
+  unsigned char* keep = smem + kStages * St::kBytes;  // KEEP: E's pieces, up to three of 16 KB
+  Bars& bar = *reinterpret_cast<Bars*>(keep + (KEEP ? kKeep : 0));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int h = blockIdx.x, n = blockIdx.y, gr = h / (p.H / p.G);
   const Seq q = seq_at(p, n);
@@ -101,6 +108,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.qs, 1);
     mbar_init(&bar.pu, 1);
     mbar_init(&bar.out_sync, kOut);
+    mbar_init(&bar.ek, kEpi);
+    mbar_init(&bar.ekfree, 1);
     mbar_init(&bar.drain, 1);
     bar.fail = 0;
     fence_mbar_init();
@@ -143,6 +152,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (c < nc)  // failed: the copies in flight land before the block ends
         for (int i = max(0, c - kStages); i < c; ++i) mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, status);
+    }
+    if (KEEP && warp == kStore && lane == 0) {  // ---- E's pieces
+      for (int c = 0; c < nc && wait1(&bar.ek, c & 1); ++c) {
+        bulk_s2g(w.E + (static_cast<long long>(q.slot + c) * p.H + h) * 3 * token_piece(p.V), keep, 3 * VP * 128);
+        bulk_commit();
+        bulk_wait_read_all();
+        mbar_arrive(&bar.ekfree);
+      }
+      bulk_wait_all();
     }
     if (warp == kMma) {  // ---- MMAs
       constexpr uint32_t id64 = tc::idesc_bf16(128, 64, false, false);
@@ -411,13 +429,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st16u(tb + tl + cKS + 32 * hf + 16, lo);
         tc::tmem_wait_st();
         arrive(&bar.u);
-        if (KEEP && row < VP) {  // E's image, while the state product runs
-          const long long ch = static_cast<long long>(q.slot + c) * p.H + h;
-          float* img = w.E + ch * token_image(p.V);
+        if (KEEP) {  // E's pieces, while the state product runs: staged, then out in one copy
+          if (c > 0 && !wait(&bar.ekfree, (c - 1) & 1)) break;
+          if (row < VP) {
+            const int pc = VP * 128;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(img + image_at(VP, row, 8 * hf + i)) =
-                make_float4(e[2 * i].x, e[2 * i].y, e[2 * i + 1].x, e[2 * i + 1].y);
+            for (int i = 0; i < 4; ++i) {
+              uint32_t m[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) split3(e[4 * i + k], hi[k], m[k], lo[k]);
+              unsigned char* to = keep + tc::chunk_off(row, 4 * hf + i);
+              *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4*>(to + pc) = make_uint4(m[0], m[1], m[2], m[3]);
+              *reinterpret_cast<uint4*>(to + 2 * pc) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.ek);
         }
       }
       // S = exp(b_end) S + (w U) K
@@ -455,7 +484,8 @@ template <int K, bool KEEP>
 cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mq, const CUtensorMap& mv, const Params& p,
                    const TcBuffers& w, uint32_t* status, cudaStream_t st) {
   static unsigned long long mask = 0;
-  const int bytes = kStages * Stage<K>::kBytes + static_cast<int>(sizeof(Bars));
+  constexpr int bytes = kStages * Stage<K>::kBytes + (KEEP ? kKeep : 0) + static_cast<int>(sizeof(Bars));
+  static_assert(bytes <= kMaxDynSmem, "shared memory");
   const cudaError_t e = static_cast<cudaError_t>(
       ensure_smem_attr(reinterpret_cast<const void*>(fwd_tc_kernel<K, KEEP>), bytes, &mask));
   if (e != cudaSuccess) return e;

@@ -11,17 +11,22 @@
 // and what the gates need, by transposed butterflies over the lanes of fp32 values:
 //   dbeta_j = sum of y over its column + w_j k_j . a3_j
 //   dg_t = sum over rows of (prefix of beta y up to t) + sum_{i >= t} r_i + sum_{j < t} c_j + exp(b_end) <dS1, S0>
-// dg and dbeta are fp32 results, and sums that cancel: S0, dS1 and E enter as three bf16 pieces each, dX as two (dv and the
-// rest), with all products of them down to 2^-24.  N is a pair where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are
+// dg and dbeta are fp32 results, and sums that cancel: S0, dS1 and E enter as three bf16 pieces each, dX as two (dv and
+// the rest), with all products of them down to 2^-24.  N is a pair where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are
 // single bf16.
 //
-// One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  S0, dS1, E
-// and dX come as fp32 images; warps 8-11 take them through registers, sum <dS1, S0> on the way and stage the pieces, S0 and
-// dS1 in steps of 16 value channels (one MMA step) through a ring of four.  Bound: the images' bytes (S0 and dS1 are 2 x 64
-// KB a chunk and head at 128 x 128), and near it the tensor pipe (about 7500 cycles a head) and the epilogues.  Roles: warps
-// 0-7 epilogues (lane quarter w % 4, column half w / 4), warps 8-11 staging, warp 12 the MMAs, warp 13 the loads of Q, K, dO
-// and dv, warp 14 dg and dbeta from the epilogues' sums.  The long loops are kept rolled where they can be: at twice the
-// code the block ran at a third of the speed, waiting for instructions.
+// One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  E's pieces
+// and dX's come as operand tiles, a head ahead.  S0 and dS1 come as fp32 images; warps 8-11 take them through registers in
+// steps of 16 value channels (one MMA step), sum <dS1, S0> on the way and write the pieces to tensor memory as the left
+// operand: a step whose left operand is there takes 14 + N / 2 cycles, from shared memory 48 + N / 2, and the pieces need
+// neither 48 KB nor a proxy fence.  (Through shared memory, with E as fp32 too, the kernel took 700 us at 4 x 4096 x 32
+// heads of 128 x 128; so, 565.)  Order of a head: F; the steps, and half-way the Q and K products of a new group, whose
+// tiles arrive late; a4 and a5.  The next head's F runs under this one's epilogue of a1 to a3.  Bound: the staging warps, 8
+// steps of about 1500 cycles of loads, turns, splits and hand-overs a head, near 17000 in all; the tensor pipe has 9500, the
+// epilogues 10000, and the bytes (S0 and dS1 are 2 x 64 KB) would allow 9000.  Roles: warps 0-7 epilogues (lane quarter
+// w % 4, column half w / 4), warps 8-11 staging, warp 12 the MMAs, warp 13 the loads, warp 14 dg and dbeta from the
+// epilogues' sums.  The long loops are kept rolled where they can be: at twice the code the block ran at a third of the
+// speed, waiting for instructions.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -39,21 +44,24 @@ constexpr int kMma = 12, kLoad = 13, kGates = 14;  // (15 only fills its warpgro
 constexpr int kThreads = 16 * 32;
 constexpr int kRegEpi = 152, kRegAux = 128, kRegCtl = 80;
 static_assert(2 * kRegEpi + kRegAux + kRegCtl == 4 * 128 && kRegAux >= 128 && kRegCtl <= 128, "register split");
-constexpr int kRing = 4;
+constexpr int kRing = 2;
 constexpr int kReg = 128 * 128;  // two 64-row tiles of 64 columns, one over the other
 
 // tensor-memory columns
 constexpr uint32_t cKQ = 0;     // [qk; kk]
-constexpr uint32_t cF = 64;     // [f; F'] of E hi and lo, of E mid, of dX lo (its rows alone); then a4 and a5
-constexpr uint32_t cA = 256;    // a1, a2
-constexpr uint32_t cA3 = 384;   // a3 of E hi and lo, of E mid
+constexpr uint32_t cF = 64;     // [f; F']; then a4
+constexpr uint32_t cFX = 128;   // F' of dX lo (its rows alone); then a5
+constexpr uint32_t cA = 192;    // a1, a2
+constexpr uint32_t cA3 = 320;   // a3
+constexpr uint32_t cRing = 384; // 16 value channels of S0, then of dS1, state columns as lanes: hi, mid, lo (8 columns each)
+constexpr uint32_t kSlot = 48;
 
 struct Bars {
-  uint64_t qk_full, qk_empty, ox_full, ox_empty, ex_full, ex_empty;
-  uint64_t s_full[kRing], s_empty[kRing];  // 16 value channels of S0 (even slots) or dS1 (odd)
+  uint64_t qk_full, qk_empty, ox_full, ox_empty, ex_full[2], ex_empty[2];
+  uint64_t s_full[kRing], s_empty[kRing];  // 16 value channels of S0 and dS1
   uint64_t g_full[2], g_empty[2];
-  uint64_t f, a, a45;          // MMA groups done
-  uint64_t nm, free;           // N, M written; all accumulators read
+  uint64_t f, a45;             // MMA groups done
+  uint64_t nm, free_f, free_a; // N, M written; a4 and a5, a1 to a3 read
   uint64_t sums, fin;          // the epilogues' sums and <dS1, S0> written; dg, dbeta done with them
   uint64_t epi_sync;           // meeting of the epilogue warps (bounded, unlike a barrier instruction)
   uint64_t drain;
@@ -71,39 +79,14 @@ struct Small {
 // Offsets from the 1024-byte aligned base.
 template <int K, int VP>
 struct Layout {
-  static constexpr int kPiece = 16 * K * 2;     // 16 state rows of one piece: a 2 KB tile per 64 columns
-  static constexpr int kStep = 3 * kPiece;      // hi, mid, lo of S0 or dS1
   static constexpr int ox = (K / 64) * kReg;             // after [Q; K]
-  static constexpr int ex = ox + (VP / 64) * kReg;       // E hi, mid, lo, dX lo
-  static constexpr int ring = ex + 4 * VP * 128;
-  static constexpr int nm = ring + kRing * kStep;        // N, M
+  static constexpr int ex = ox + (VP / 64) * kReg;       // E hi, mid, lo, dX lo, of this head and the next
+  static constexpr int kEx = 4 * VP * 128;
+  static constexpr int nm = ex + 2 * kEx;                // N, M
   static constexpr int out = nm + 2 * kTile;             // N lo; 32 rows of dq or dk on their way out
   static constexpr int small = out + kTile;              // (32 x dstate bf16 fit it)
   static constexpr int bytes = small + static_cast<int>(sizeof(Small));
 };
-
-// Columns 8 chunk .. 8 chunk + 7 of a row of an fp32 image.
-__device__ __forceinline__ void load_row8(const float* img, int VP, int row, int chunk, float2 (&v)[4]) {
-  const float4 a = __ldcs(reinterpret_cast<const float4*>(img + image_at(VP, row, 2 * chunk)));
-  const float4 b = __ldcs(reinterpret_cast<const float4*>(img + image_at(VP, row, 2 * chunk + 1)));
-  v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
-}
-// Their three pieces as 16-byte chunks at `to`, `stride` bytes apart.
-__device__ __forceinline__ void stage_row8(unsigned char* to, int stride, const float2 (&v)[4]) {
-  uint32_t h[4], m[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) split3(v[i], h[i], m[i], l[i]);
-  *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-  *reinterpret_cast<uint4*>(to + stride) = make_uint4(m[0], m[1], m[2], m[3]);
-  *reinterpret_cast<uint4*>(to + 2 * stride) = make_uint4(l[0], l[1], l[2], l[3]);
-}
-// The second piece alone.
-__device__ __forceinline__ void stage_lo8(unsigned char* to, const float2 (&v)[4]) {
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) split2(v[i], h[i], l[i]);
-  *reinterpret_cast<uint4*>(to) = make_uint4(l[0], l[1], l[2], l[3]);
-}
 
 // Sums of 16 columns over the warp's 32 lanes: lane l gets column l / 2.
 __device__ __forceinline__ float column_sums(float (&x)[16], int lane) {
@@ -117,6 +100,15 @@ __device__ __forceinline__ float column_sums(float (&x)[16], int lane) {
     }
   }
   return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 1);
+}
+
+// Four lanes' 4 x 4 turned: lane j of them gives element i to lane i's place j.
+__device__ __forceinline__ float4 turn4(float4 v, int lane) {
+  const bool b0 = (lane & 1) != 0, b1 = (lane & 2) != 0;
+  const float g0 = __shfl_xor_sync(0xffffffffu, b0 ? v.x : v.y, 1), g1 = __shfl_xor_sync(0xffffffffu, b0 ? v.z : v.w, 1);
+  v = b0 ? make_float4(g0, v.y, g1, v.w) : make_float4(v.x, g0, v.z, g1);
+  const float h0 = __shfl_xor_sync(0xffffffffu, b1 ? v.x : v.z, 2), h1 = __shfl_xor_sync(0xffffffffu, b1 ? v.y : v.w, 2);
+  return b1 ? make_float4(h0, h1, v.z, v.w) : make_float4(v.x, v.y, h0, h1);
 }
 
 template <int K, int VP>
@@ -135,15 +127,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile uint32_t* fail = &bar.fail;
 
   if (tid == 0) {
-    uint64_t* one[] = {&bar.qk_full, &bar.ox_full, &bar.ox_empty, &bar.ex_empty, &bar.s_empty[0], &bar.s_empty[1],
-                       &bar.s_empty[2], &bar.s_empty[3], &bar.g_full[0], &bar.g_full[1], &bar.f, &bar.a, &bar.a45, &bar.fin, &bar.drain};
+    uint64_t* one[] = {&bar.qk_full, &bar.ox_full, &bar.ox_empty, &bar.ex_full[0], &bar.ex_full[1], &bar.ex_empty[0],
+                       &bar.ex_empty[1], &bar.s_empty[0], &bar.s_empty[1], &bar.g_full[0], &bar.g_full[1], &bar.f,
+                       &bar.a45, &bar.fin, &bar.drain};
     for (uint64_t* b : one) mbar_init(b, 1);
     mbar_init(&bar.qk_empty, 1 + kEpi);
-    mbar_init(&bar.ex_full, kAux);
     for (int i = 0; i < kRing; ++i) mbar_init(&bar.s_full[i], kAux);
     for (int i = 0; i < 2; ++i) mbar_init(&bar.g_empty[i], kEpi + 1);
     mbar_init(&bar.nm, kEpi);
-    mbar_init(&bar.free, kEpi);
+    mbar_init(&bar.free_f, kEpi);
+    mbar_init(&bar.free_a, kEpi);
     mbar_init(&bar.sums, kEpi + kAux);
     mbar_init(&bar.epi_sync, kEpi);
     bar.fail = 0;
@@ -180,28 +173,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int slot = t / p.G, gr = t - slot * p.G;
         if (!chunk_at(p, slot, &n, &q, &tok)) continue;
         const int tt = q.t0 + tok;
-        if (task > 0 && !(ok = wait1(&bar.qk_empty, (task - 1) & 1))) break;
-        mbar_arrive_expect_tx(&bar.qk_full, (K / 64) * kReg);
-        for (int i = 0; i < K / 64; ++i) {
-          tma_load_4d(smem + i * kReg, &mq, &bar.qk_full, 64 * i, gr, tt, q.b);
-          tma_load_4d(smem + i * kReg + kTile, &mk, &bar.qk_full, 64 * i, gr, tt, q.b);
-        }
-        ++task;
         for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
           const long long ch = static_cast<long long>(slot) * p.H + h;
           const uint32_t last = (hc - 1) & 1;
-          bulk_prefetch_l2(w.E + ch * token_image(p.V), VP * kC * 4);  // warps 8-11 read these next
-          bulk_prefetch_l2(w.dX + ch * token_image(p.V), VP * kC * 4);
-          bulk_prefetch_l2(w.S + ch * state_image(p.V, K), VP * K * 4);
+          bulk_prefetch_l2(w.S + ch * state_image(p.V, K), VP * K * 4);  // warps 8-11 read these next
           bulk_prefetch_l2(w.dS + ch * state_image(p.V, K), VP * K * 4);
+          for (int i = 0; i < VP / 64; ++i) {
+            tma_prefetch_4d(&mo, 64 * i, h, tt, q.b);
+            tma_prefetch_4d(&mdv, 64 * i, h, tt, q.b);
+          }
           if (hc > 1 && !(ok = wait1(&bar.g_empty[hc & 1], (hc / 2 - 1) & 1))) break;
           mbar_arrive_expect_tx(&bar.g_full[hc & 1], kGateFloats * 4);
           bulk_g2s(sm.gate[hc & 1], w.gates + ch * kGateFloats, kGateFloats * 4, &bar.g_full[hc & 1]);
+          if (hc > 1 && !(ok = wait1(&bar.ex_empty[hc & 1], (hc / 2 - 1) & 1))) break;
+          mbar_arrive_expect_tx(&bar.ex_full[hc & 1], 4 * img);
+          unsigned char* ex = smem + Lay::ex + (hc & 1) * Lay::kEx;
+          bulk_g2s(ex, w.E + ch * 3 * img, 3 * img, &bar.ex_full[hc & 1]);
+          bulk_g2s(ex + 3 * img, w.dX + ch * img, img, &bar.ex_full[hc & 1]);
           if (hc > 0 && !(ok = wait1(&bar.ox_empty, last))) break;
           mbar_arrive_expect_tx(&bar.ox_full, (VP / 64) * kReg);
           for (int i = 0; i < VP / 64; ++i) {
             tma_load_4d(smem + Lay::ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
             tma_load_4d(smem + Lay::ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
+          }
+          if (h == gr * hpg) {  // Q and K, which the products with E do not need
+            if (task > 0 && !(ok = wait1(&bar.qk_empty, (task - 1) & 1))) break;
+            mbar_arrive_expect_tx(&bar.qk_full, (K / 64) * kReg);
+            for (int i = 0; i < K / 64; ++i) {
+              tma_load_4d(smem + i * kReg, &mq, &bar.qk_full, 64 * i, gr, tt, q.b);
+              tma_load_4d(smem + i * kReg + kTile, &mk, &bar.qk_full, 64 * i, gr, tt, q.b);
+            }
+            ++task;
           }
         }
       }
@@ -212,10 +214,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == kMma) {  // ---- MMAs
       constexpr uint32_t idKQ = tc::idesc_bf16(128, 64, false, false);
-      constexpr uint32_t idF = tc::idesc_bf16(128, 128, false, true);
-      constexpr uint32_t idF64 = tc::idesc_bf16(128, 64, false, true);
-      constexpr uint32_t idA = tc::idesc_bf16(128, 128, true, false);
-      constexpr uint32_t idMM128 = tc::idesc_bf16(128, 128, true, true);
+      constexpr uint32_t idF = tc::idesc_bf16(128, 64, false, true);
+      constexpr uint32_t idA = tc::idesc_bf16(128, 128, false, false);
+      constexpr uint32_t idA64 = tc::idesc_bf16(128, 64, false, true);
       constexpr uint32_t idMM = tc::idesc_bf16(128, 64, true, true);
       constexpr uint32_t idMK = tc::idesc_bf16(128, 64, true, false);
       auto kstep = [](int s) { return static_cast<uint32_t>(((s >> 2) * kReg + (s & 3) * 32) >> 4); };
@@ -223,18 +224,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto jstep = [](int s) { return static_cast<uint32_t>((s * 32) >> 4); };
       const uint32_t sb = smem_u32(smem);
       // state columns as lanes: two 64-column regions (dstate 64: the same one twice, the upper lanes are not read)
-      constexpr uint32_t sreg = K == 128 ? 2048u : 0u, qreg = K == 128 ? kReg : 0u;
+      constexpr uint32_t qreg = K == 128 ? kReg : 0u;
       const uint32_t dQK = desc_lo(sb, 16), dK = desc_lo(sb + kTile, 16);
       const uint32_t dQn = desc_lo(sb, qreg), dKn = desc_lo(sb + kTile, qreg);
       const uint32_t dOX = desc_lo(sb + Lay::ox, 16);
-      const uint32_t dE = desc_lo(sb + Lay::ex, img);            // [E hi | E mid]
-      const uint32_t dEm = desc_lo(sb + Lay::ex + img, img);     // E mid
-      const uint32_t dEl = desc_lo(sb + Lay::ex + 2 * img, img); // E lo
-      const uint32_t dEX = desc_lo(sb + Lay::ex, 3 * img);       // [E hi | dX lo]
-      const uint32_t dXl = desc_lo(sb + Lay::ex + 3 * img, img);
-      const uint32_t dRing = desc_lo(sb + Lay::ring, sreg);
       const uint32_t dN = desc_lo(sb + Lay::nm, 16), dM = desc_lo(sb + Lay::nm + kTile, 16);
       const uint32_t dNl = desc_lo(sb + Lay::out, 16);
+      constexpr uint32_t im = img >> 4;  // from one piece of E to the next
       int n, tok, task = 0, hc = 0, rc = 0;
       Seq q;
       bool ok = true;
@@ -243,18 +239,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!chunk_at(p, slot, &n, &q, &tok)) continue;
         const int have = q.len - tok;
         const bool cut = have < kC && p.cu != nullptr;  // rows of the next sequence in the tiles
-        ok = wait(&bar.qk_full, task & 1);
-        if (!ok) break;
-        if (cut) {
-          zero_rows(smem, K / 64, kReg, have);
-          zero_rows(smem + kTile, K / 64, kReg, have);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        ++task;
         for (int h = 0; h < hpg; ++h, ++hc) {
           const uint32_t ph = hc & 1;
-          ok = wait(&bar.ox_full, ph) && wait(&bar.ex_full, ph);
+          const uint32_t dE = desc_lo(sb + Lay::ex, img) + ph * (Lay::kEx >> 4);       // E hi, mid, lo, dX lo
+          const uint32_t dEX = desc_lo(sb + Lay::ex, 3 * img) + ph * (Lay::kEx >> 4);  // [E hi | dX lo]
+          ok = wait(&bar.ox_full, ph) && wait(&bar.ex_full[ph], (hc >> 1) & 1);
           if (!ok) break;
           if (cut) {
             zero_rows(smem + Lay::ox, VP / 64, kReg, have);
@@ -262,14 +251,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_proxy_async_smem();
             __syncwarp();
           }
-          if (hc > 0) ok = wait(&bar.free, (hc - 1) & 1);
+          if (hc > 0) ok = wait(&bar.free_f, (hc - 1) & 1);
           if (!ok) break;
           tc::fence_after_sync();
           if (elect_one()) {
-            if (h == 0) {
-#pragma unroll 1
-              for (int s = 0; s < K / 16; ++s) mma_ss(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
-            }
 #pragma unroll 1
             for (int s4 = 0; s4 < steps / 4; ++s4) {  // 64 value channels
               const uint32_t ox = dOX + s4 * (kReg >> 4), vo = s4 * 512;
@@ -277,50 +262,67 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 4; ++i) {
                 const bool more = s4 > 0 || i > 0;
                 mma_ss(tb + cF, ox + 2 * i, dE + vo + 128 * i, idF, more);
-                mma_ss(tb + cF, ox + 2 * i, dEl + vo + 128 * i, idF64, true);
-                mma_ss(tb + cF + 128, dEX + vo + 128 * i, dE + vo + 128 * i, idMM, more);
-                mma_ss(tb + cF + 128, dEX + vo + 128 * i, dEm + vo + 128 * i, idMM, true);
+                mma_ss(tb + cF, ox + 2 * i, dE + im + vo + 128 * i, idF, true);
+                mma_ss(tb + cF, ox + 2 * i, dE + 2 * im + vo + 128 * i, idF, true);
+                mma_ss(tb + cFX, dEX + vo + 128 * i, dE + vo + 128 * i, idMM, more);
+                mma_ss(tb + cFX, dEX + vo + 128 * i, dE + im + vo + 128 * i, idMM, true);
               }
             }
-            tc::mma_commit(&bar.f);
           }
           __syncwarp();
+          if (h > 0 && elect_one()) tc::mma_commit(&bar.f);
+          __syncwarp();
+          if (hc > 0) ok = wait(&bar.free_a, (hc - 1) & 1);
 #pragma unroll 1
-          for (int s2 = 0; ok && s2 < steps / 2; ++s2, ++rc) {  // the ring once around: two steps, S0 and dS1 of each
+          for (int s2 = 0; ok && s2 < steps / 2; ++s2, ++rc) {  // the ring once around
+            if (h == 0 && s2 == steps / 4) {  // Q K^t and K K^t, late: Q and K come when the last group is done with theirs
+              ok = wait(&bar.qk_full, task & 1);
+              if (!ok) break;
+              if (cut) {
+                zero_rows(smem, K / 64, kReg, have);
+                zero_rows(smem + kTile, K / 64, kReg, have);
+                fence_proxy_async_smem();
+                __syncwarp();
+              }
+              ++task;
+              if (elect_one()) {
+#pragma unroll 1
+                for (int s = 0; s < K / 16; ++s) mma_ss(tb + cKQ, dQK + kstep(s), dK + kstep(s), idKQ, s > 0);
+                tc::mma_commit(&bar.f);
+              }
+              __syncwarp();
+            }
             const uint32_t ox = dOX + (s2 >> 1) * (kReg >> 4) + (s2 & 1) * 4, vo = s2 * 256;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              constexpr uint32_t pc = Lay::kPiece >> 4, slot16 = Lay::kStep >> 4;
-              const uint32_t dS = dRing + 2 * i * slot16, dD = dS + slot16;
+              constexpr uint32_t pc = kSlot / 6;
+              const uint32_t aS = tb + cRing + i * kSlot, aD = aS + 3 * pc;
+              const uint32_t e = dE + vo + 128 * i;
               const bool more = s2 > 0 || i > 0;
-              ok = ok && wait(&bar.s_full[2 * i], rc & 1);
+              ok = ok && wait(&bar.s_full[i], rc & 1);
               if (!ok) break;
+              tc::fence_after_sync();
               if (elect_one()) {
-                mma_ss(tb + cA, dS, ox + 2 * i, idA, more);
-                mma_ss(tb + cA, dS + pc, ox + 2 * i, idA, true);
-                mma_ss(tb + cA, dS + 2 * pc, ox + 2 * i, idA, true);
-                mma_ss(tb + cA + 64, dS, dXl + vo + 128 * i, idMM, true);
-                mma_ss(tb + cA + 64, dS + pc, dXl + vo + 128 * i, idMM, true);
-                tc::mma_commit(&bar.s_empty[2 * i]);
-              }
-              __syncwarp();
-              ok = wait(&bar.s_full[2 * i + 1], rc & 1);
-              if (!ok) break;
-              if (elect_one()) {
-                mma_ss(tb + cA3, dD, dE + vo + 128 * i, idMM128, more);
-                mma_ss(tb + cA3, dD + pc, dE + vo + 128 * i, idMM128, true);
-                mma_ss(tb + cA3, dD, dEl + vo + 128 * i, idMM, true);
-                mma_ss(tb + cA3, dD + 2 * pc, dE + vo + 128 * i, idMM, true);
-                tc::mma_commit(&bar.s_empty[2 * i + 1]);
+                mma_ts_lo(tb + cA, aS, ox + 2 * i, idA, more);
+                mma_ts_lo(tb + cA, aS + pc, ox + 2 * i, idA, true);
+                mma_ts_lo(tb + cA, aS + 2 * pc, ox + 2 * i, idA, true);
+                mma_ts_lo(tb + cA + 64, aS, e + 3 * im, idA64, true);
+                mma_ts_lo(tb + cA + 64, aS + pc, e + 3 * im, idA64, true);
+                mma_ts_lo(tb + cA3, aD, e, idA64, more);
+                mma_ts_lo(tb + cA3, aD + pc, e, idA64, true);
+                mma_ts_lo(tb + cA3, aD + 2 * pc, e, idA64, true);
+                mma_ts_lo(tb + cA3, aD, e + im, idA64, true);
+                mma_ts_lo(tb + cA3, aD + pc, e + im, idA64, true);
+                mma_ts_lo(tb + cA3, aD, e + 2 * im, idA64, true);
+                tc::mma_commit(&bar.s_empty[i]);
               }
               __syncwarp();
             }
           }
           if (!ok) break;
           if (elect_one()) {
-            tc::mma_commit(&bar.a);
             tc::mma_commit(&bar.ox_empty);
-            tc::mma_commit(&bar.ex_empty);
+            tc::mma_commit(&bar.ex_empty[ph]);
           }
           __syncwarp();
           ok = wait(&bar.nm, ph);
@@ -331,11 +333,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int s = 0; s < 4; ++s) {
               mma_ss(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
               mma_ss(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
-              mma_ss(tb + cF + 64, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
-              mma_ss(tb + cF + 64, dKn + nstep(s), dM + nstep(s), idMM, true);
-              mma_ss(tb + cF + 64, dQn + nstep(s), dN + nstep(s), idMM, true);
+              mma_ss(tb + cFX, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
+              mma_ss(tb + cFX, dKn + nstep(s), dM + nstep(s), idMM, true);
+              mma_ss(tb + cFX, dQn + nstep(s), dN + nstep(s), idMM, true);
             }
-            tc::mma_commit(&bar.a45);
+            tc::mma_commit(&bar.a45);  // and with them a1 to a3
             if (h == hpg - 1) tc::mma_commit(&bar.qk_empty);
           }
           __syncwarp();
@@ -406,88 +408,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= kEpi) {  // ---- staging, <dS1, S0>
     set_regs_up<kRegAux>();
-    const int at = tid - kEpi * 32;
+    const int quarter = warp & 3;
+    const bool staging = 32 * quarter < K;  // (dstate 64: the upper lanes of S0 and dS1 hold nothing and are not read)
     int n, tok, hc = 0, rc = 0;
     Seq q;
     bool ok = true;
-    auto publish = [&](uint64_t* b) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b);
-    };
     for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
       const int slot = t / p.G, gr = t - slot * p.G;
       if (!chunk_at(p, slot, &n, &q, &tok)) continue;
       for (int h = gr * hpg; h < (gr + 1) * hpg; ++h, ++hc) {
         const long long ch = static_cast<long long>(slot) * p.H + h;
-        const float *gE = w.E + ch * token_image(p.V), *gX = w.dX + ch * token_image(p.V);
         const float *gS = w.S + ch * state_image(p.V, K), *gD = w.dS + ch * state_image(p.V, K);
-        // E and dX: 8 chunks of 8 tokens per row, two of each in flight; the first steps of S0 and dS1 on their way meanwhile
-        float2 e[2][4], x[2][4];
-        const int row = at & (VP - 1), c0 = VP == 128 ? 0 : at >> 6, cs = VP == 128 ? 1 : 2;
-        auto fetch2 = [&](int c) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            load_row8(gE, VP, row, c + k * cs, e[k]);
-            load_row8(gX, VP, row, c + k * cs, x[k]);
-          }
-        };
-        // S0 and dS1, 16 rows a step: K / 8 chunks per row, two steps in flight
+        // S0 and dS1, 16 value channels a step, two steps in flight.  A thread's lane is a state column; four lanes load
+        // four columns of four channels, four times, and turn them among themselves.
         float2 acc = make_float2(0, 0);
-        constexpr int kItems = 16 * (K / 8) / (kAux * 32);  // chunks of a thread and step: 1 (dstate 64) or 2
-        float2 s0[2][kItems][4], d1[2][kItems][4];
+        float4 s0[2][4], d1[2][4];
+        const int piece = 8 * quarter + (lane >> 2);
         auto fetch = [&](int s, int into) {
+          if (staging) {
 #pragma unroll
-          for (int k = 0; k < kItems; ++k) {
-            const int i = at + k * kAux * 32;
-            load_row8(gS, VP, 16 * s + (i & 15), i >> 4, s0[into][k]);
-            load_row8(gD, VP, 16 * s + (i & 15), i >> 4, d1[into][k]);
+            for (int m = 0; m < 4; ++m) {
+              s0[into][m] = __ldcs(reinterpret_cast<const float4*>(gS + image_at(VP, 16 * s + 4 * m + (lane & 3), piece)));
+              d1[into][m] = __ldcs(reinterpret_cast<const float4*>(gD + image_at(VP, 16 * s + 4 * m + (lane & 3), piece)));
+            }
           }
         };
-        fetch2(c0);
-        fetch(0, 0);
-        ok = hc == 0 || wait(&bar.ex_empty, (hc - 1) & 1);
-        if (!ok) break;
-#pragma unroll 1
-        for (int c = c0; c < 8; c += 2 * cs) {
+        auto put = [&](float4 (&f)[4], uint32_t to) {
+          uint32_t o[24];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            unsigned char* to = smem + Lay::ex + tc::chunk_off(row, c + k * cs);
-            stage_row8(to, img, e[k]);
-            stage_lo8(to + 3 * img, x[k]);  // dX hi is dv
+          for (int m = 0; m < 4; ++m) {
+            const float4 v = turn4(f[m], lane);
+            split3(make_float2(v.x, v.y), o[2 * m], o[8 + 2 * m], o[16 + 2 * m]);
+            split3(make_float2(v.z, v.w), o[2 * m + 1], o[9 + 2 * m], o[17 + 2 * m]);
           }
-          if (c + 2 * cs < 8) fetch2(c + 2 * cs);
-        }
-        publish(&bar.ex_full);
+          tmem_st16u(to, o);
+          tmem_st8u(to + 16, o + 16);
+        };
+        fetch(0, 0);
         fetch(1, 1);
 #pragma unroll 1
         for (int s2 = 0; ok && s2 < steps; s2 += 2, ++rc) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            ok = ok && (rc == 0 || wait(&bar.s_empty[2 * u], (rc - 1) & 1));
+            ok = ok && (rc == 0 || wait(&bar.s_empty[u], (rc - 1) & 1));
             if (!ok) break;
-            unsigned char* base = smem + Lay::ring + 2 * u * Lay::kStep;
+            tc::fence_after_sync();
+            if (staging) {
+              const uint32_t to = tb + cRing + u * kSlot + (static_cast<uint32_t>(32 * quarter) << 16);
 #pragma unroll
-            for (int k = 0; k < kItems; ++k) {
-              const int i = at + k * kAux * 32, r = i & 15, c = i >> 4;
-#pragma unroll
-              for (int m = 0; m < 4; ++m) acc = f2_fma(s0[u][k][m], d1[u][k][m], acc);
-              stage_row8(base + (c >> 3) * 2048 + tc::chunk_off(r, c & 7), Lay::kPiece, s0[u][k]);
+              for (int m = 0; m < 4; ++m) {
+                acc = f2_fma(make_float2(s0[u][m].x, s0[u][m].y), make_float2(d1[u][m].x, d1[u][m].y), acc);
+                acc = f2_fma(make_float2(s0[u][m].z, s0[u][m].w), make_float2(d1[u][m].z, d1[u][m].w), acc);
+              }
+              put(s0[u], to);
+              put(d1[u], to + kSlot / 2);
+              tc::tmem_wait_st();
             }
-            publish(&bar.s_full[2 * u]);
-            ok = rc == 0 || wait(&bar.s_empty[2 * u + 1], (rc - 1) & 1);
-            if (!ok) break;
-#pragma unroll
-            for (int k = 0; k < kItems; ++k) {
-              const int i = at + k * kAux * 32, r = i & 15, c = i >> 4;
-              stage_row8(base + Lay::kStep + (c >> 3) * 2048 + tc::chunk_off(r, c & 7), Lay::kPiece, d1[u][k]);
-            }
-            publish(&bar.s_full[2 * u + 1]);
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.s_full[u]);
             if (s2 + 2 < steps) fetch(s2 + 2 + u, u);
           }
         }
         if (!ok) break;
-        float d = acc.x + acc.y;
+        float d = staging ? acc.x + acc.y : 0.f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
         ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
@@ -527,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         {  // rows: f and qk (lanes 0-63), F' and kk (64-127); columns c0 .., 16 at a time
           const int i = row & 63;
           const bool second = quarter >= 2;
-          const float own = second ? 1.f : 0.f;  // (the upper rows of the third part are E E^t)
+          const float own = second ? 1.f : 0.f;  // (the upper rows of cFX are E E^t)
           const float bi = gate[kGateB + i], sc = second ? -1.f : p.scale;
           const uint32_t wide = __float_as_uint(gate[kGateWide]);
           unsigned char* tile = smem + Lay::nm + (second ? kTile : 0);
@@ -539,13 +523,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int cg = c0 + 16 * g, lim = (second ? i - 1 : i) - cg;  // last of these columns in the row
             float x[16];
             {
-              float a[16], b[16];
+              float b[16];
               tc::tmem_ld16(tb + tl + cF + cg, x);
-              tc::tmem_ld16(tb + tl + cF + 64 + cg, a);
-              tc::tmem_ld16(tb + tl + cF + 128 + cg, b);
+              tc::tmem_ld16(tb + tl + cFX + cg, b);
               tc::tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 16; ++k) x[k] = fmaf(own, b[k], x[k] + a[k]);
+              for (int k = 0; k < 16; ++k) x[k] = fmaf(own, b[k], x[k]);
             }
             if ((wide >> (cg / 2)) & 1u) {  // bit 8 of a 16-token group
 #pragma unroll
@@ -599,10 +582,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_smem();
           arrive(&bar.nm);
         }
-        // state columns as lanes: a1, a2, a3
-        ok = wait(&bar.a, ph);
+        // state columns as lanes: a4, a5, whose place the next head waits for; then a1, a2, a3
+        ok = wait(&bar.a45, ph);
         if (!ok) break;
         tc::fence_after_sync();
+        {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float a[16], b[16];
+            tc::tmem_ld16(tb + tl + cF + c0 + 16 * g, a);
+            tc::tmem_ld16(tb + tl + cFX + c0 + 16 * g, b);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              dq[16 * g + k] += a[k];
+              dk[16 * g + k] += b[k];
+            }
+          }
+        }
+        arrive(&bar.free_f);
         {
           // (dstate 64: lanes 64 and above hold nothing; they read the lower lanes' elements and count for nothing)
           const unsigned char* tq = smem + (K == 128 ? (row >> 6) * kReg : 0) + c0 * 128;
@@ -613,12 +611,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const int cg = c0 + 16 * g;
-            float s[16], kv[16], a[16], b[16];
+            float s[16], kv[16], a[16], b[16], a3[16];
             tc::tmem_ld16(tb + tl + cA + cg, a);
             tc::tmem_ld16(tb + tl + cA + 64 + cg, b);
+            tc::tmem_ld16(tb + tl + cA3 + cg, a3);
 #pragma unroll
             for (int k = 0; k < 16; ++k) kv[k] = elem(tq + kTile, 16 * g + k);
             tc::tmem_wait_ld();
+            if (g == 1) arrive(&bar.free_a);
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
               const float2 e = *reinterpret_cast<const float2*>(gate + kGateE + cg + k);
@@ -636,14 +636,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 16; ++k) s[k] = 0.f;
             }
             const float r = column_sums(s, lane);
-            tc::tmem_ld16(tb + tl + cA3 + cg, a);
-            tc::tmem_ld16(tb + tl + cA3 + 64 + cg, b);
-            tc::tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
               const float2 bw = *reinterpret_cast<const float2*>(gate + kGateW + cg + k);
               const float2 wt = *reinterpret_cast<const float2*>(gate + kGateTail + cg + k);
-              const float v0 = a[k] + b[k], v1 = a[k + 1] + b[k + 1];
+              const float v0 = a3[k], v1 = a3[k + 1];
               dk[16 * g + k] = fmaf(bw.x, v0, dk[16 * g + k]);
               dk[16 * g + k + 1] = fmaf(bw.y, v1, dk[16 * g + k + 1]);
               s[k] = wt.x * v0 * kv[k];
@@ -665,24 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&bar.sums);
           mbar_arrive(&bar.g_empty[hc & 1]);
         }
-        ok = wait(&bar.a45, ph);
-        if (!ok) break;
-        tc::fence_after_sync();
-        {
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float a[16], b[16];
-            tc::tmem_ld16(tb + tl + cF + c0 + 16 * g, a);
-            tc::tmem_ld16(tb + tl + cF + 64 + c0 + 16 * g, b);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              dq[16 * g + k] += a[k];
-              dk[16 * g + k] += b[k];
-            }
-          }
-        }
-        arrive(&bar.free);
       }
       if (!ok) break;
       if (lane == 0) mbar_arrive(&bar.qk_empty);  // (its tiles were last read before bar.sums)

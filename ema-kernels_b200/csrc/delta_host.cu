@@ -58,14 +58,14 @@ size_t carve_tc_fwd(TcBuffers* w, char* base, int64_t slots, int64_t H, int64_t 
   w->T = c.bytes(n * 2 * kTile);
   w->P = c.bytes(n * 2 * kTile);
   w->S = keep ? c.take(n * state_image(static_cast<int>(V), static_cast<int>(K))) : nullptr;
-  w->E = keep ? c.take(n * token_image(static_cast<int>(V))) : nullptr;
+  w->E = keep ? c.bytes(n * 3 * token_piece(static_cast<int>(V))) : nullptr;
   return c.at;
 }
 size_t carve_tc_bwd(TcBuffers* w, char* base, int64_t slots, int64_t H, int64_t V, int64_t K) {
   Carver c{base};
   const size_t n = static_cast<size_t>(slots) * H;
   w->dS = c.take(n * state_image(static_cast<int>(V), static_cast<int>(K)));
-  w->dX = c.take(n * token_image(static_cast<int>(V)));
+  w->dX = c.bytes(n * token_piece(static_cast<int>(V)));
   return c.at;
 }
 // The tensor-core kernels take bf16 (every dstate and headdim of the entry points); a call without tokens, whose

@@ -9,8 +9,9 @@
 //
 // Images.  T and P lie in global memory as the 128-byte swizzled bf16 tiles that shared memory wants (rows of 64 bf16,
 // 16-byte chunk c of row r at c ^ (r % 8)), so that a plain bulk copy stages them: 64 x 64, row = token i, column =
-// token j, hi then lo (8 KB each).  S, dS, E and dX are fp32, for a thread that owns the row of a value channel:
-// four columns after four columns, each with all the rows, so that a warp stores and loads 512 bytes in a piece.
+// token j, hi then lo (8 KB each); E and dX likewise, row = value channel, column = token, one piece after another.
+// S and dS are fp32, for a thread that owns the row of a value channel: four columns after four columns, each with all
+// the rows, so that a warp stores 512 bytes at a time.
 #pragma once
 
 #include "delta_common.cuh"
@@ -35,15 +36,16 @@ struct TcBuffers {
   char* T;           // T - I: hi, lo
   char* P;           // hi, lo
   float* S;          // state entering the chunk (null: not kept)
-  float* E;          // (null: not kept)
+  char* E;           // hi, mid, lo (null: not kept)
   float* dS;         // gradient of the state at the chunk's end
-  float* dX;
+  char* dX;          // lo alone: dv is its hi
 };
 
 __host__ __device__ inline int pad_channels(int V) { return V <= 64 ? 64 : 128; }
 // Floats of an image, and the place of columns 4 piece .. 4 piece + 3 of a row in it.
 __host__ __device__ inline size_t state_image(int V, int K) { return static_cast<size_t>(pad_channels(V)) * K; }
-__host__ __device__ inline size_t token_image(int V) { return static_cast<size_t>(pad_channels(V)) * kC; }
+// Bytes of one piece of E or dX.
+__host__ __device__ inline size_t token_piece(int V) { return static_cast<size_t>(pad_channels(V)) * kC * 2; }
 __device__ __forceinline__ int image_at(int VP, int row, int piece) { return (piece * VP + row) * 4; }
 
 // bf16 pair (x, y) -> packed hi and packed lo.
@@ -95,7 +97,22 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo,
       : "memory");
 }
 
-// 32 lanes x 16 columns of raw 32-bit words.
+__device__ __forceinline__ void mma_ts_lo(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(kDescHi)
+      : "memory");
+}
+
+// 32 lanes x 8 and x 16 columns of raw 32-bit words.
+__device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -103,6 +120,18 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+// A tile on its way to the L2 cache.
+__device__ __forceinline__ void tma_prefetch_4d(const void* map, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(y), "r"(z),
+               "r"(w)
+               : "memory");
+}
+// Shared to global memory; the caller commits and waits.
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src_smem, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src_smem)), "r"(bytes)
+               : "memory");
 }
 
 // A warpgroup's share of the registers the block was launched with; all its warps call it.  N is at least (up), at
