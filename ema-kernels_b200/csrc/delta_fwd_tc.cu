@@ -11,8 +11,8 @@
 // for E and U P^t; w U, whose rounding stays in the state, is three pieces.  (o = scale exp(b) S Q^t + U P^t ends in bf16, but where keys repeat its two terms
 // cancel: hi parts alone left it 1e-2 off there.)
 //
-// Bound: the chain's latency, 6100 cycles a chunk at dstate 128 (16384 tokens of 32 heads of 128: 850 us; 40 sequences, 8111
-// tokens of 16 heads: 118): three dependent MMA groups (about 1000, 640 and 950 cycles) with an epilogue after each (600,
+// Bound: the chain's latency, 6000 cycles a chunk at dstate 128 (16384 tokens of 32 heads of 128: 825 us, and 850 with the
+// state product in one piece; 40 sequences, 8111 tokens of 16 heads: 116): three dependent MMA groups (about 1000, 640 and 950 cycles) with an epilogue after each (600,
 // 750 and 980) and the hand-overs between them; the products for o run in their shadow.  A training forward with a block on
 // most SMs is near its bytes instead: it writes S, E and o, 128 KB a chunk and head (4 x 4096 x 32: 310 us, 3.6 TB/s of writes
 // and 0.9 of reads).  Roles: warps 0-7 the chain's epilogues
@@ -53,8 +53,8 @@ constexpr uint32_t cSl = 448;  // S lo
 
 struct Bars {
   uint64_t full[kStages], empty[kStages];
-  uint64_t ks, qs, e, ds, pu;  // MMA groups done
-  uint64_t s, x, wu, u;    // epilogues done: state, X, w U and U ready
+  uint64_t ks, qs, e, ds[2], pu;  // MMA groups done (ds: 64 state columns each)
+  uint64_t s[2], x, wu, u;  // epilogues done: state (64 columns each), X, w U and U ready
   uint64_t q, o;           // Q S, U P read
   uint64_t ek, ekfree;     // E's pieces staged, and on their way to memory
   uint64_t out_sync;       // meeting of the output warps (bounded, unlike a barrier instruction)
@@ -98,8 +98,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bar.ks, 1);
     mbar_init(&bar.e, 1);
-    mbar_init(&bar.ds, 1);
-    mbar_init(&bar.s, kEpi);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.ds[i], 1);
+      mbar_init(&bar.s[i], kEpi);
+    }
     mbar_init(&bar.x, kEpi);
     mbar_init(&bar.wu, kEpi);
     mbar_init(&bar.u, kEpi);
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMma) {  // ---- MMAs
       constexpr uint32_t id64 = tc::idesc_bf16(128, 64, false, false);
       constexpr uint32_t id128 = tc::idesc_bf16(128, 128, false, false);
-      constexpr uint32_t idK = tc::idesc_bf16(128, K, false, true);
+      constexpr uint32_t idK = tc::idesc_bf16(128, 64, false, true);
       for (int c = 0; c < nc; ++c) {
         const int st = c % kStages;
         unsigned char* base = smem + st * St::kBytes;
@@ -179,9 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (ok && c > 0) ok = wait(&bar.pu, (c - 1) & 1);  // U has been read where K S lands
-        ok = ok && wait(&bar.s, c & 1);
         if (!ok) break;
-        tc::fence_after_sync();
         const uint64_t dq = tc::smem_desc_sw128(sb + St::oKQ, 16, 1024);
         const uint64_t dk = tc::smem_desc_sw128(sb + St::oKQ + kTile, 16, 1024);
         const uint64_t dkn = tc::smem_desc_sw128(sb + St::oKQ + kTile, kReg, 1024);
@@ -192,14 +192,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto jstep = [](int s) { return static_cast<uint64_t>((s * 32) >> 4); };
         auto nstep = [](int s) { return static_cast<uint64_t>((s * 2048) >> 4); };
         auto ucol = [](int s) { return static_cast<uint32_t>((s >> 1) * 32 + (s & 1) * 8); };
-        if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < K / 16; ++s) mma_ts(tb + cKS, tb + cSh + 8 * s, dk + kstep(s), id64, s > 0);
+        for (int g = 0; g < K / 64; ++g) {
+          ok = ok && wait(&bar.s[g], c & 1);
+          if (!ok) break;
+          tc::fence_after_sync();
+          if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < K / 16; ++s) mma_ts(tb + cKS, tb + cSl + 8 * s, dk + kstep(s), id64, true);
-          tc::mma_commit(&bar.ks);
+            for (int s = 4 * g; s < 4 * g + 4; ++s) mma_ts(tb + cKS, tb + cSh + 8 * s, dk + kstep(s), id64, s > 0);
+#pragma unroll
+            for (int s = 4 * g; s < 4 * g + 4; ++s) mma_ts(tb + cKS, tb + cSl + 8 * s, dk + kstep(s), id64, true);
+            if (g == K / 64 - 1) tc::mma_commit(&bar.ks);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         if (elect_one()) {
 #pragma unroll
           for (int s = 0; s < K / 16; ++s) mma_ts(tb + cDS, tb + cSh + 8 * s, dq + kstep(s), id64, s > 0);
@@ -223,12 +230,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cX + 8 * s, dkn + nstep(s), idK, s > 0);
+          for (int g = 0; g < K / 64; ++g) {  // a tile of K each, so that the first columns' epilogue starts earlier
+            const uint64_t kg = dkn + ((g * kReg) >> 4);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cX + 32 + 8 * s, dkn + nstep(s), idK, true);
+            for (int s = 0; s < 4; ++s) mma_ts(tb + cDS + 64 * g, tb + cX + 8 * s, kg + nstep(s), idK, s > 0);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) mma_ts(tb + cDS, tb + cX + 64 + 8 * s, dkn + nstep(s), idK, true);
-          tc::mma_commit(&bar.ds);
+            for (int s = 0; s < 4; ++s) mma_ts(tb + cDS + 64 * g, tb + cX + 32 + 8 * s, kg + nstep(s), idK, true);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) mma_ts(tb + cDS + 64 * g, tb + cX + 64 + 8 * s, kg + nstep(s), idK, true);
+            tc::mma_commit(&bar.ds[g]);
+          }
         }
         __syncwarp();
         if (!wait(&bar.u, c & 1)) break;
@@ -323,15 +334,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {  // ---- the chain's epilogues
     set_regs_up<kRegEpi>();
-    constexpr int KC = K / 2;  // state columns of a thread
+    constexpr int KC = K / 2;  // state columns of a thread: 32 hf .. of each 64
     const int row = 32 * (warp & 3) + lane, hf = warp >> 2;
     const uint32_t tl = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const bool live = row < p.V;
     float2 S[KC / 2];
-    const long long srow = ((static_cast<long long>(n) * p.H + h) * p.V + row) * K + hf * KC;
+    const long long srow = ((static_cast<long long>(n) * p.H + h) * p.V + row) * K + 32 * hf;
 #pragma unroll
     for (int i = 0; i < KC; i += 4) {
-      const float4 f = (live && p.s0 != nullptr) ? *reinterpret_cast<const float4*>(p.s0 + srow + i)
+      const float4 f = (live && p.s0 != nullptr) ? *reinterpret_cast<const float4*>(p.s0 + srow + i + (i & 32))
                                                   : make_float4(0, 0, 0, 0);
       S[i / 2] = make_float2(f.x, f.y), S[i / 2 + 1] = make_float2(f.z, f.w);
     }
@@ -340,26 +351,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
-    // the state as hi / lo operand columns
-    auto publish = [&]() {
+    // 32 columns of the state as hi / lo operand columns
+    auto publish = [&](int g) {
+      uint32_t hi[16], lo[16];
 #pragma unroll
-      for (int g = 0; g < KC / 32; ++g) {
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) split2(S[16 * g + i], hi[i], lo[i]);
-        tmem_st16u(tb + tl + cSh + hf * (KC / 2) + 16 * g, hi);
-        tmem_st16u(tb + tl + cSl + hf * (KC / 2) + 16 * g, lo);
-      }
+      for (int i = 0; i < 16; ++i) split2(S[16 * g + i], hi[i], lo[i]);
+      tmem_st16u(tb + tl + cSh + 32 * g + 16 * hf, hi);
+      tmem_st16u(tb + tl + cSl + 32 * g + 16 * hf, lo);
       tc::tmem_wait_st();
+      arrive(&bar.s[g]);
     };
+#pragma unroll
+    for (int g = 0; g < KC / 32; ++g) publish(g);
     for (int c = 0; c < nc; ++c) {
-      publish();
-      arrive(&bar.s);
       if (KEEP && row < VP) {
         float* img = w.S + (static_cast<long long>(q.slot + c) * p.H + h) * state_image(p.V, K);
 #pragma unroll
         for (int i = 0; i < KC / 4; ++i)
-          *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
+          *reinterpret_cast<float4*>(img + image_at(VP, row, 8 * hf + i + (i & 8))) =
               make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
       }
       const int st = c % kStages;
@@ -450,25 +459,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // S = exp(b_end) S + (w U) K
-      if (!wait(&bar.ds, c & 1)) break;
-      tc::fence_after_sync();
       const float dec = gate[kGateEnd];
+      bool ok = true;
 #pragma unroll
       for (int g = 0; g < KC / 32; ++g) {
+        ok = ok && wait(&bar.ds[g], c & 1);
+        if (!ok) break;
+        tc::fence_after_sync();
         float a[2][16];
-        tc::tmem_ld16(tb + tl + cDS + hf * KC + 32 * g, a[0]);
-        tc::tmem_ld16(tb + tl + cDS + hf * KC + 32 * g + 16, a[1]);
+        tc::tmem_ld16(tb + tl + cDS + 64 * g + 32 * hf, a[0]);
+        tc::tmem_ld16(tb + tl + cDS + 64 * g + 32 * hf + 16, a[1]);
         tc::tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 16; ++i) S[16 * g + i] = f2_fma(f2_bcast(dec), S[16 * g + i], pair(a, i));
+        publish(g);
       }
+      if (!ok) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.empty[st]);
     }
     if (live && p.s1 != nullptr) {
 #pragma unroll
       for (int i = 0; i < KC; i += 4)
-        *reinterpret_cast<float4*>(p.s1 + srow + i) =
+        *reinterpret_cast<float4*>(p.s1 + srow + i + (i & 32)) =
             make_float4(S[i / 2].x, S[i / 2].y, S[i / 2 + 1].x, S[i / 2 + 1].y);
     }
   }
