@@ -10,9 +10,10 @@
 // pairs (delta_tc.cuh), dO~, whose rounding stays in dS, three pieces.  dv = dX; for the gradient kernel dS at every chunk's
 // end is left as an fp32 image, and what dX has beyond dv as a bf16 tile.
 //
-// Bound: the chain's latency, as in the forward walk (three dependent MMA groups of about 900, 750 and 950 cycles
-// with their hand-overs, and an epilogue after each): 280 us at 4 x 4096 tokens of 32 heads of 128 x 128.  Roles: warps 0-7 the chain's epilogues, warps 8-11 dO~ and the
-// copy of dv to its rows, warp 12 the MMAs, warp 13 the loads.
+// Bound: the chain's latency, as in the forward walk (three dependent MMA groups of about 900, 750 and 950 cycles with
+// their hand-overs, and an epilogue after each): 264 us at 4 x 4096 tokens of 32 heads of 128 x 128, 175 on 9 packed
+// sequences of 8 heads.  dS's image leaves in parts, one in every gap of the chain (at once: 283).  Roles: warps 0-7 the
+// chain's epilogues, warps 8-11 dO~ and the copy of dv to its rows, warp 12 the MMAs, warp 13 the loads.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -321,13 +322,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
       }
       arrive(&bar.s);
-      if (row < VP) {
-        float* img = w.dS + ch * state_image(p.V, K);
+      // dS's image in parts
+      auto keep_state = [&](int from, int to) {
+        if (row < VP) {
+          float* img = w.dS + ch * state_image(p.V, K);
 #pragma unroll
-        for (int i = 0; i < KC / 4; ++i)
-          *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
-              make_float4(D[2 * i].x, D[2 * i].y, D[2 * i + 1].x, D[2 * i + 1].y);
-      }
+          for (int i = 0; i < KC / 4; ++i)
+            if (i >= from && i < to)
+              *reinterpret_cast<float4*>(img + image_at(VP, row, hf * KC / 4 + i)) =
+                  make_float4(D[2 * i].x, D[2 * i].y, D[2 * i + 1].x, D[2 * i + 1].y);
+        }
+      };
+      keep_state(0, 3 * KC / 32);
       if (!wait(&bar.full[st], (r / kStages) & 1) || !wait(&bar.z, r & 1)) break;
       tc::fence_after_sync();
       float2 x[16];  // W, then dX
@@ -351,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
       }
       arrive(&bar.w);
+      keep_state(3 * KC / 32, 3 * KC / 16);
       if (!wait(&bar.dx, r & 1)) break;
       tc::fence_after_sync();
       {
@@ -395,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.dv);
       }
+      keep_state(3 * KC / 16, KC / 4);
       if (!wait(&bar.ds, r & 1)) break;
       tc::fence_after_sync();
       const float dec = gate[kGateEnd];

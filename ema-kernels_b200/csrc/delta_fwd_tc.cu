@@ -8,17 +8,17 @@
 // is a chain of M = 128 MMAs whose left operand (S, X, U) the epilogue threads write straight back to tensor memory
 // -- no shared-memory round trip and no transpose -- and whose right operands K, Q, T, P are the tiles as
 // loaded.  Operands that are not bf16 by nature are hi + lo pairs (delta_tc.cuh): 2 products for S K^t and S Q^t, 3
-// for E and U P^t; w U, whose rounding stays in the state, is three pieces.  (o = scale exp(b) S Q^t + U P^t ends in bf16, but where keys repeat its two terms
-// cancel: hi parts alone left it 1e-2 off there.)
+// for E and U P^t; w U, whose rounding stays in the state, is three pieces.  (o = scale exp(b) S Q^t
+// + U P^t ends in bf16, but where keys repeat its two terms cancel: hi parts alone left it 1e-2 off there.)
 //
 // Bound: the chain's latency, 6000 cycles a chunk at dstate 128 (16384 tokens of 32 heads of 128: 825 us, and 850 with the
-// state product in one piece; 40 sequences, 8111 tokens of 16 heads: 116): three dependent MMA groups (about 1000, 640 and 950 cycles) with an epilogue after each (600,
-// 750 and 980) and the hand-overs between them; the products for o run in their shadow.  A training forward with a block on
-// most SMs is near its bytes instead: it writes S, E and o, 128 KB a chunk and head (4 x 4096 x 32: 310 us, 3.6 TB/s of writes
-// and 0.9 of reads).  Roles: warps 0-7 the chain's epilogues
-// (warp w: lanes 32 (w % 4), half w / 4 of the columns; the fp32 state lives in their registers), warps 8-11 the
-// output, warp 12 issues the MMAs, warp 13 the loads (TMA for K, Q, V; bulk copies for the images), two stages deep, warp
-// 14 E's copies to memory.
+// state product in one piece; 40 sequences, 8111 tokens of 16 heads: 116): three
+// dependent MMA groups (about 1000, 640 and 950 cycles) with an epilogue after each (600, 750 and 980) and the hand-overs
+// between them; the products for o run in their shadow.  A training forward with a block on most SMs is near its bytes
+// instead: it writes S, E and o, 128 KB a chunk and head, and reads 96 (4 x 4096 x 32: 320 us, 5.8 TB/s; 250 without S).
+// Roles: warps 0-7 the chain's epilogues (warp w: lanes 32 (w % 4), 32 (w / 4) .. of every 64 columns; the fp32 state lives
+// in their registers), warps 8-11 the output, warp 12 issues the MMAs, warp 13 the loads (TMA for K, Q, V; bulk copies for
+// the images), two stages deep, warp 14 E's copies to memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -364,13 +364,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int g = 0; g < KC / 32; ++g) publish(g);
     for (int c = 0; c < nc; ++c) {
-      if (KEEP && row < VP) {
-        float* img = w.S + (static_cast<long long>(q.slot + c) * p.H + h) * state_image(p.V, K);
+      // KEEP: the state's image, a part in every gap of the chain (all at once the stores hold up the loads behind them)
+      auto keep_state = [&](int from, int to) {
+        if (KEEP && row < VP) {
+          float* img = w.S + (static_cast<long long>(q.slot + c) * p.H + h) * state_image(p.V, K);
 #pragma unroll
-        for (int i = 0; i < KC / 4; ++i)
-          *reinterpret_cast<float4*>(img + image_at(VP, row, 8 * hf + i + (i & 8))) =
-              make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
-      }
+          for (int i = 0; i < KC / 4; ++i)
+            if (i >= from && i < to)
+              *reinterpret_cast<float4*>(img + image_at(VP, row, 8 * hf + i + (i & 8))) =
+                  make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
+        }
+      };
       const int st = c % kStages;
       const unsigned char* base = smem + st * St::kBytes;
       const float* gate = reinterpret_cast<const float*>(base + St::oG);
@@ -385,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = (live && 32 * hf + i < have) ? v[i] : 0.f;
       }
+      keep_state(0, KC / 16);
       if (!wait(&bar.ks, c & 1)) break;
       tc::fence_after_sync();
       float2 x[16];
@@ -405,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
       }
       arrive(&bar.x);
+      keep_state(KC / 16, 3 * KC / 16);
       // U = beta E; first w U, which the state waits for
       if (!wait(&bar.e, c & 1)) break;
       tc::fence_after_sync();
@@ -459,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // S = exp(b_end) S + (w U) K
+      keep_state(3 * KC / 16, KC / 4);
       const float dec = gate[kGateEnd];
       bool ok = true;
 #pragma unroll

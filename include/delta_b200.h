@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-/* bf16 calls run on the tensor cores, their 32-bit operands as pairs of bf16 (2^-17 of each); with this flag
+/* bf16 calls run on the tensor cores, their 32-bit operands as two or three bf16 pieces (2^-16 of each); with this flag
  * their products are fp32 on the CUDA cores, as those of fp16 and fp32 calls always are. */
 #define DELTA_FP32_PRODUCTS 1
 
