@@ -150,10 +150,11 @@ __device__ __forceinline__ void write_partial(const Params& p, const float (&dw)
   }
 }
 
-// grid: (row blocks, groups of a row).  One norm row per group of TG threads and iteration; the next row's loads are
-// issued before this one's arithmetic (raw, so a 16-bit tensor costs four registers a vector), which is what keeps enough
-// bytes in flight: without it the gated pair at 8192 x 32 heads of 128 took 202 and 396 us; with it,
-// 156 and 261 (6.6 and 6.2 TB/s), the residual pair at 32768 x 2048 139 and 181.
+// grid: (row blocks, groups of a row).  One norm row per group of TG threads at a time; the loads of the next two rows
+// (of the next one where a row is longer) are issued before a row's arithmetic, raw, so that a 16-bit tensor costs four
+// registers a vector: the bytes in flight are what bounds it.  The gated pair at 8192 x 32 heads of 128: 202 and 396 us
+// without, 156 and 261 one row ahead, 146 and 251 two (5.5 and 5.3 TB/s; packed arithmetic, two channels an instruction,
+// made no difference); the residual pair at 32768 x 2048: 131 and 176 (6.1 TB/s).
 // FIRST: the norm comes before the gate.
 template <class T, class R, int TG, int VEC, int NV, bool RES, bool BWD, bool FIRST>
 __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? (BWD ? 2 : 3) : 1) norm_kernel(const Params p) {
@@ -177,13 +178,18 @@ __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? 
       dw[j][k] = 0.f;
     }
   constexpr int NG = kThreads / TG;
-  // (long rows have enough bytes in flight by themselves, and no registers for two)
-  constexpr bool kAhead = NV * VEC * static_cast<int>(sizeof(T)) <= 32;
+  // rows loaded ahead (long rows have enough bytes in flight by themselves, and no registers for more)
+  constexpr int kBytes = NV * VEC * static_cast<int>(sizeof(T)), kAhead = kBytes <= 16 && VEC > 1 ? 2 : kBytes <= 32 ? 1 : 0;
   const long long step = static_cast<long long>(gridDim.x) * NG;
-  Raw<TA, VEC> ra[NV];
-  Raw<TB, VEC> rb[NV];
-  Raw<T, VEC> rc[NV];
-  auto fetch = [&](long long row, Raw<TA, VEC> (&a)[NV], Raw<TB, VEC> (&b)[NV], Raw<T, VEC> (&d)[NV]) {
+  struct Row {
+    Raw<TA, VEC> a[NV];
+    Raw<TB, VEC> b[NV];
+    Raw<T, VEC> d[NV];
+  };
+  auto fetch = [&](long long row, Row& in) {
+    auto &a = in.a;
+    auto &b = in.b;
+    auto &d = in.d;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * TG + lane) * VEC;
@@ -200,16 +206,12 @@ __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? 
         for (int k = 0; k < VEC; ++k) b[j].e[k] = from_f32<TB>(0.f);
     }
   };
-  if (kAhead) fetch(static_cast<long long>(blockIdx.x) * NG + grp, ra, rb, rc);
-  // every thread of a warp takes part in the shuffles of every iteration: a group without a row adds zeros
-  for (long long r0 = static_cast<long long>(blockIdx.x) * NG; r0 < p.rows; r0 += step) {
-    const long long row = r0 + grp;
+  // every thread of a warp takes part in the shuffles of every row: a group without one (past the end) adds zeros
+  auto work = [&](long long row, const Row& in) {
+    const auto &ra = in.a;
+    const auto &rb = in.b;
+    const auto &rc = in.d;
     const bool live = row < p.rows;
-    Raw<TA, VEC> na[NV];
-    Raw<TB, VEC> nb[NV];
-    Raw<T, VEC> nd[NV];
-    if (!kAhead) fetch(row, ra, rb, rc);
-    else if (r0 + step < p.rows) fetch(row + step, na, nb, nd);
     float t[NV][VEC], sg[NV][VEC];  // the normed value, the gate's sigmoid
     float sum = 0.f, dot = 0.f;
 #pragma unroll
@@ -272,11 +274,35 @@ __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? 
           if (RES && p.dz != nullptr) store_v<R, VEC>(static_cast<R*>(p.dz) + row * p.sdz + g0 + c, p.aligned, b);
         }
       }
-      if (kAhead) {
-        ra[j] = na[j];
-        rb[j] = nb[j];
-        if (BWD) rc[j] = nd[j];
-      }
+    }
+  };
+  long long row = static_cast<long long>(blockIdx.x) * NG + grp;
+  if constexpr (kAhead == 2) {
+    Row r0, r1, r2;
+    fetch(row, r0);
+    fetch(row + step, r1);
+    for (; row - grp < p.rows; row += 3 * step) {
+      fetch(row + 2 * step, r2);
+      work(row, r0);
+      fetch(row + 3 * step, r0);
+      work(row + step, r1);
+      fetch(row + 4 * step, r1);
+      work(row + 2 * step, r2);
+    }
+  } else if constexpr (kAhead == 1) {
+    Row r0, r1;
+    fetch(row, r0);
+    for (; row - grp < p.rows; row += 2 * step) {
+      fetch(row + step, r1);
+      work(row, r0);
+      fetch(row + 2 * step, r0);
+      work(row + step, r1);
+    }
+  } else {
+    for (; row - grp < p.rows; row += step) {
+      Row r0;
+      fetch(row, r0);
+      work(row, r0);
     }
   }
   if constexpr (BWD) write_partial<TG, VEC, NV>(p, dw, lane, grp);
