@@ -240,7 +240,7 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
     all sums and both gate gradients are fp32.  bf16 calls run on the tensor cores with their 32-bit operands as
     pairs or threes of bf16: 2^-16 of each, some 4e-6 of a state or gate gradient.  Where keys repeat and beta is near one,
     the gate gradients are small differences of large terms and keep fewer digits; ``fp32_products`` then gives
-    those of fp32 arithmetic, at about twenty times the time.  fp16 and fp32 calls are always fp32 products."""
+    those of fp32 arithmetic, at about seventeen times the time.  fp16 and fp32 calls are always fp32 products."""
     b, length, H, V, G, K = _check(q, k, v, g, beta, "gated_delta_rule")
     _check_headdim(V, 128, "gated_delta_rule")
     nseq = b

@@ -132,7 +132,7 @@ def test_repeated_keys(dt):
 
 
 def test_repeated_keys_on_operand_pairs():
-    """The same on the tensor cores.  Their operand pairs hold 2^-17 of a value where fp32 holds 2^-24, so the gate
+    """The same on the tensor cores.  Their operand pairs hold 2^-17 of a value on average where fp32 holds 2^-24, so the gate
     gradients, differences of sums of up to 32 x 32 (dg) and 64 (dbeta) products of the size scale |do| |v|, may be off
     by 2^-17 of the root of the sum of squares of those products; everything else holds its tolerance."""
     def edit(x):
