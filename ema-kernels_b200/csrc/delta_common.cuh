@@ -40,6 +40,8 @@ namespace delta {
 
 constexpr int kC = 64;              // tokens of a chunk
 constexpr float kMinGate = -100.f;  // exp(-100) = 4e-44: a reset; keeps differences of running sums finite
+// (not fmaxf, which would make a reset of a gate that is no number)
+__device__ __forceinline__ float clamp_gate(float g) { return g < kMinGate ? kMinGate : g; }
 
 struct View {
   long long b, t, h;  // element strides of batch, token, head / group

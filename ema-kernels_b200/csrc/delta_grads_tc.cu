@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int j = 2 * lane + k;
             if (tok + j < q.len) {
               const long long to = (static_cast<long long>(q.b) * p.L + q.t0 + tok + j) * p.H + h;
-              p.dg[to] = p.g[to] > kMinGate ? dg[k] : 0.f;  // a clamped gate has no gradient
+              p.dg[to] = p.g[to] <= kMinGate ? 0.f : dg[k];  // a clamped gate has no gradient
               p.dbeta[to] = y[k] + c[k];
             }
           }

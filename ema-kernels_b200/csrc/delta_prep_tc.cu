@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_tc_kernel(const __grid_const
     for (int k = 0; k < 2; ++k) {
       const int t = 2 * lane + k;
       const long long at = (static_cast<long long>(q.b) * p.L + q.t0 + tok + t) * p.H + h;
-      g[k] = t < have ? fmaxf(p.g[at], kMinGate) : 0.f;
+      g[k] = t < have ? clamp_gate(p.g[at]) : 0.f;
       be[k] = t < have ? p.beta[at] : 0.f;
     }
     float run = g[0] + g[1];

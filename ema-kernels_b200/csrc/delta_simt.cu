@@ -89,7 +89,7 @@ __device__ __forceinline__ void load_gates(const Params& p, const Seq& s, int to
     for (int i = 0; i < 2; ++i) {
       const int t = tok + 2 * lane + i;
       const long long at = (static_cast<long long>(s.b) * p.L + s.t0 + t) * p.H + h;
-      g[i] = t < s.len ? fmaxf(p.g[at], kMinGate) : 0.f;
+      g[i] = t < s.len ? clamp_gate(p.g[at]) : 0.f;
       be[i] = t < s.len ? p.beta[at] : 0.f;
     }
     float run = g[0] + g[1];
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
       }
       for (int j = 0; j < t; ++j) sum += sc[j];
       const long long at = (static_cast<long long>(s.b) * p.L + s.t0 + tok + t) * p.H + h;
-      p.dg[at] = p.g[at] > kMinGate ? sum : 0.f;  // a clamped gate has no gradient
+      p.dg[at] = p.g[at] <= kMinGate ? 0.f : sum;  // a clamped gate has no gradient
     }
     __syncthreads();
 #pragma unroll

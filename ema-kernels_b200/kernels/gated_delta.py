@@ -230,11 +230,12 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
                      fp32_products=False):
     """o (batch, seqlen, nheads, headdim), or (o, final states) with ``return_final_states``.
 
-    g is the log decay (not positive in a decaying layer; at or below -100 the state is dropped), beta the write
-    strength, ``scale`` defaults to dstate ** -0.5.  ``initial_states`` (sequences, nheads, headdim, dstate)
-    is the state before the first token.  ``cu_seqlens`` (nseq + 1, int32 or int64, on the device) packs
-    sequences into a batch of one: sequence n is tokens [cu[n], cu[n + 1]), of any length, zero too
-    (its final state is its initial one); tokens outside every sequence give zeros.
+    g is the log decay (not positive in a decaying layer; at or below -100 the state is dropped; a NaN makes NaN of
+    its head's results from its token on and of those before it in its chunk of 64), beta the write strength, ``scale``
+    defaults to dstate ** -0.5.  ``initial_states`` (sequences, nheads, headdim, dstate) is the state before the first
+    token.  ``cu_seqlens`` (nseq + 1, int32 or int64, on the device) packs sequences into a batch of one: sequence n is
+    tokens [cu[n], cu[n + 1]), of any length, zero too (its final state is its initial one); tokens outside every
+    sequence give zeros.
 
     Gradients: q, k, v, g, beta and initial_states; those of a group's q and k sum over its heads.  The states,
     all sums and both gate gradients are fp32.  bf16 calls run on the tensor cores with their 32-bit operands as
