@@ -39,9 +39,31 @@ namespace emab {
 namespace delta {
 
 constexpr int kC = 64;              // tokens of a chunk
-constexpr float kMinGate = -100.f;  // exp(-100) = 4e-44: a reset; keeps differences of running sums finite
+constexpr float kMinGate = -100.f;  // exp(-100) = 4e-44: a reset; keeps sums and their differences finite
 // (not fmaxf, which would make a reset of a gate that is no number)
 __device__ __forceinline__ float clamp_gate(float g) { return g < kMinGate ? kMinGate : g; }
+
+// The running sum of a chunk's gates is taken in 64 bits and kept as two floats: a decay between two tokens is a difference of
+// such sums, and in 32 bits it would have the digits of what steep gates before both have summed to (one reset in four
+// tokens: 3e-5 of o).
+struct GateSum {
+  float hi, lo;
+};
+__device__ __forceinline__ GateSum gate_sum(double b) {
+  const float hi = static_cast<float>(b);
+  return GateSum{hi, static_cast<float>(b - hi)};
+}
+__device__ __forceinline__ float operator-(GateSum a, GateSum b) { return (a.hi - b.hi) + (a.lo - b.lo); }
+// Inclusive sums of the warp's 64 gates, two a lane: up to the lane's second one.
+__device__ __forceinline__ double gate_scan(const float (&g)[2], int lane) {
+  double run = static_cast<double>(g[0]) + g[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  return run;
+}
 
 struct View {
   long long b, t, h;  // element strides of batch, token, head / group

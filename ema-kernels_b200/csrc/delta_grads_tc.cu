@@ -512,7 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int i = row & 63;
           const bool second = quarter >= 2;
           const float own = second ? 1.f : 0.f;  // (the upper rows of cFX are E E^t)
-          const float bi = gate[kGateB + i], sc = second ? -1.f : p.scale;
+          const GateSum bi = {gate[kGateB + i], gate[kGateBLo + i]};
+          const float sc = second ? -1.f : p.scale;
           const uint32_t wide = __float_as_uint(gate[kGateWide]);
           unsigned char* tile = smem + Lay::nm + (second ? kTile : 0);
           ok = hc == 0 || wait(&bar.fin, (hc - 1) & 1);  // the last head's sums have been read
@@ -532,9 +533,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if ((wide >> (cg / 2)) & 1u) {  // bit 8 of a 16-token group
 #pragma unroll
-              for (int k = 0; k < 16; ++k) x[k] *= sc * __expf(bi - gate[kGateB + cg + k]);
+              for (int k = 0; k < 16; ++k) x[k] *= sc * __expf(bi - GateSum{gate[kGateB + cg + k], gate[kGateBLo + cg + k]});
             } else {
-              const float rf = sc * __expf(bi - gate[kGateB + cg]);
+              const float rf = sc * __expf(bi - GateSum{gate[kGateB + cg], gate[kGateBLo + cg]});
 #pragma unroll
               for (int k = 0; k < 16; k += 4) {
                 const float4 k4 = *reinterpret_cast<const float4*>(gate + kGateKey + cg + k);

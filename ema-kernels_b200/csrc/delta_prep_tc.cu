@@ -34,7 +34,8 @@ struct Matrices {  // over the operand tiles, once their product is read
   float W[4][16][kWLd];
 };
 struct Shared {
-  float b[kHeads][kC], beta[kHeads][kC], key[kHeads][kC];  // key: exp(b_r - b_j), or 1 in a wide group
+  GateSum b[kHeads][kC];
+  float beta[kHeads][kC], key[kHeads][kC];  // key: exp(b_r - b_j), or 1 in a wide group
   uint32_t wide[kHeads];
   uint64_t full, mma;
   uint32_t taddr, fail;
@@ -178,35 +179,32 @@ __global__ void __launch_bounds__(kThreads, 4) prep_tc_kernel(const __grid_const
       g[k] = t < have ? clamp_gate(p.g[at]) : 0.f;
       be[k] = t < have ? p.beta[at] : 0.f;
     }
-    float run = g[0] + g[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float v = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += v;
-    }
-    const float end = __shfl_sync(0xffffffffu, run, 31);
-    const float first = __shfl_sync(0xffffffffu, run - g[1], lane & ~7);  // b of the 16-token group's first token
-    const float last = __shfl_sync(0xffffffffu, run, lane | 7);
-    const bool wide = fabsf(first - last) > kWideSpan;
+    const double run = gate_scan(g, lane), left = run - g[1];
+    const double end = __shfl_sync(0xffffffffu, run, 31);
+    const double first = __shfl_sync(0xffffffffu, left, lane & ~7);  // b of the 16-token group's first token
+    const double last = __shfl_sync(0xffffffffu, run, lane | 7);
+    const bool wide = fabs(first - last) > kWideSpan;
     const uint32_t wb = __ballot_sync(0xffffffffu, wide);
     float* rec = w.gates + (static_cast<long long>(slot) * p.H + h) * kGateFloats;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float b = k == 0 ? run - g[1] : run;
+      const double b = k == 0 ? left : run;
+      const GateSum bs = gate_sum(b);
       const int t = 2 * lane + k;
-      s.b[e][t] = b;
+      s.b[e][t] = bs;
       s.beta[e][t] = be[k];
-      const float key = wide ? 1.f : expf(first - b), tail = expf(end - b);
+      const float key = wide ? 1.f : expf(static_cast<float>(first - b)), tail = expf(static_cast<float>(end - b));
       s.key[e][t] = key;
-      rec[kGateE + t] = -expf(b);
+      rec[kGateE + t] = -expf(bs.hi);
       rec[kGateW + t] = be[k] * tail;
       rec[kGateBeta + t] = be[k];
-      rec[kGateB + t] = b;
+      rec[kGateB + t] = bs.hi;
+      rec[kGateBLo + t] = bs.lo;
       rec[kGateKey + t] = key;
       rec[kGateTail + t] = tail;
     }
     if (lane == 0) {
-      rec[kGateEnd] = expf(end);
+      rec[kGateEnd] = expf(static_cast<float>(end));
       s.wide[e] = wb;  // bit 8 g: group g
       rec[kGateWide] = __uint_as_float(wb);
     }
@@ -263,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_tc_kernel(const __grid_const
   for (int h = h0; h < h1; ++h) {
     const long long ch = static_cast<long long>(slot) * p.H + h;
     const int e = h - h0;
-    const float bi = s.b[e][i];
+    const GateSum bi = s.b[e][i];
     const uint32_t wide = s.wide[e];
     char* hi = w.P + ch * 2 * kTile;
 #pragma unroll

@@ -81,7 +81,7 @@ __device__ __forceinline__ void load_flat(float* dst, int stride, const float* s
 }
 
 // The chunk's gates: b (running sums), beta; both zero-extended past the sequence (b stays at its last value).
-__device__ __forceinline__ void load_gates(const Params& p, const Seq& s, int tok, int h, float* sb, float* sbeta) {
+__device__ __forceinline__ void load_gates(const Params& p, const Seq& s, int tok, int h, GateSum* sb, float* sbeta) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     float g[2], be[2];
@@ -92,14 +92,9 @@ __device__ __forceinline__ void load_gates(const Params& p, const Seq& s, int to
       g[i] = t < s.len ? clamp_gate(p.g[at]) : 0.f;
       be[i] = t < s.len ? p.beta[at] : 0.f;
     }
-    float run = g[0] + g[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float v = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += v;
-    }
-    sb[2 * lane] = run - g[1];
-    sb[2 * lane + 1] = run;
+    const double run = gate_scan(g, lane);
+    sb[2 * lane] = gate_sum(run - g[1]);
+    sb[2 * lane + 1] = gate_sum(run);
     sbeta[2 * lane] = be[0];
     sbeta[2 * lane + 1] = be[1];
   }
@@ -113,8 +108,8 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Params p, const Bu
   float* sq = sk + kC * ks;
   float* sa = sq + kC * ks;
   float* st = sa + kC * kS;
-  float* sb = st + kC * kS;
-  float* sbeta = sb + kC;
+  GateSum* sb = reinterpret_cast<GateSum*>(st + kC * kS);
+  float* sbeta = reinterpret_cast<float*>(sb + kC);
   const int slot = blockIdx.x, h = blockIdx.y, gr = h / (p.H / p.G);
   int n, tok;
   Seq s;
@@ -155,8 +150,8 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Params p, const Buf
   float* sp = st + kC * kS;
   float* sx = sp + kC * kS;       // X, then U
   float* su = sx + kC * kVS;
-  float* sb = su + kC * kVS;
-  float* sbeta = sb + kC;
+  GateSum* sb = reinterpret_cast<GateSum*>(su + kC * kVS);
+  float* sbeta = reinterpret_cast<float*>(sb + kC);
   const int v0 = blockIdx.x * kVB, h = blockIdx.y, n = blockIdx.z, gr = h / (p.H / p.G);
   const Seq s = seq_at(p, n);
   const int have = min(kVB, p.V - v0);
@@ -181,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Params p, const Buf
     float acc[4][2];
     zero(acc);
     product(acc, K, [&](int i, int kk) { return sk[i * ks + kk]; }, [&](int kk, int j) { return ss[j * ks + kk]; });
-    each(acc, [&](int i, int j, float v) { sx[i * kVS + j] = fmaf(-expf(sb[i]), v, sx[i * kVS + j]); });
+    each(acc, [&](int i, int j, float v) { sx[i * kVS + j] = fmaf(-expf(sb[i].hi), v, sx[i * kVS + j]); });
     __syncthreads();
     zero(acc);
     product(acc, kC, [&](int i, int kk) { return st[i * kS + kk]; }, [&](int kk, int j) { return sx[kk * kVS + j]; });
@@ -191,14 +186,14 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Params p, const Buf
     });
     zero(acc);
     product(acc, K, [&](int i, int kk) { return sq[i * ks + kk]; }, [&](int kk, int j) { return ss[j * ks + kk]; });
-    each(acc, [&](int i, int j, float& v) { v *= p.scale * expf(sb[i]); });
+    each(acc, [&](int i, int j, float& v) { v *= p.scale * expf(sb[i].hi); });
     __syncthreads();
     product(acc, kC, [&](int i, int kk) { return sp[i * kS + kk]; }, [&](int kk, int j) { return su[kk * kVS + j]; });
     each(acc, [&](int i, int j, float v) {
       if (tok + i < s.len && j < have)
         row_of<T>(p.o, p.vo, s.b, s.t0 + tok + i, h)[v0 + j] = from_f32<T>(v);
     });
-    const float end = sb[kC - 1];
+    const GateSum end = sb[kC - 1];
     for (int i = threadIdx.x; i < kC * K; i += kThreads) {
       const int r = i / K, c = i - r * K;
       sk[r * ks + c] *= expf(end - sb[r]);
@@ -207,7 +202,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Params p, const Buf
     float up[2][KJ];
     zero(up);
     product(up, kC, [&](int i, int kk) { return su[kk * kVS + i]; }, [&](int kk, int j) { return sk[kk * ks + j]; });
-    const float dec = expf(end);
+    const float dec = expf(end.hi);
     each(up, [&](int i, int j, float v) { ss[i * ks + j] = fmaf(dec, ss[i * ks + j], v); });
   }
   __syncthreads();
@@ -226,8 +221,8 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Params p, const Buf
   float* sp = st + kC * kS;
   float* so = sp + kC * kS;       // dO
   float* su = so + kC * kVS;      // beta dU, then dX
-  float* sb = su + kC * kVS;
-  float* sbeta = sb + kC;
+  GateSum* sb = reinterpret_cast<GateSum*>(su + kC * kVS);
+  float* sbeta = reinterpret_cast<float*>(sb + kC);
   const int v0 = blockIdx.x * kVB, h = blockIdx.y, n = blockIdx.z, gr = h / (p.H / p.G);
   const Seq s = seq_at(p, n);
   const int have = min(kVB, p.V - v0);
@@ -248,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Params p, const Buf
     for (int i = threadIdx.x; i < have * K; i += kThreads)
       w.dS1[ch * p.V * K + v0 * K + i] = ss[(i / K) * ks + i % K];
     __syncthreads();
-    const float end = sb[kC - 1];
+    const GateSum end = sb[kC - 1];
     float acc[4][2];
     zero(acc);
     product(acc, K, [&](int i, int kk) { return sk[i * ks + kk]; }, [&](int kk, int j) { return ss[j * ks + kk]; });
@@ -263,8 +258,8 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Params p, const Buf
     product(acc, kC, [&](int i, int kk) { return st[kk * kS + i]; }, [&](int kk, int j) { return su[kk * kVS + j]; });
     __syncthreads();
     each(acc, [&](int i, int j, float v) {
-      su[i * kVS + j] = v * -expf(sb[i]);
-      so[i * kVS + j] *= p.scale * expf(sb[i]);
+      su[i * kVS + j] = v * -expf(sb[i].hi);
+      so[i * kVS + j] *= p.scale * expf(sb[i].hi);
       if (j < have) {
         w.dX[(ch * kC + i) * p.V + v0 + j] = v;
         if (tok + i < s.len) row_of<T>(p.dv, p.vdv, s.b, s.t0 + tok + i, h)[v0 + j] = from_f32<T>(v);
@@ -275,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Params p, const Buf
     zero(up);
     product(up, kC, [&](int i, int kk) { return so[kk * kVS + i]; }, [&](int kk, int j) { return sq[kk * ks + j]; });
     product(up, kC, [&](int i, int kk) { return su[kk * kVS + i]; }, [&](int kk, int j) { return sk[kk * ks + j]; });
-    const float dec = expf(end);
+    const float dec = expf(end.hi);
     each(up, [&](int i, int j, float v) { ss[i * ks + j] = fmaf(dec, ss[i * ks + j], v); });
   }
   __syncthreads();
@@ -303,8 +298,8 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
   float* se = sx + kC * kVS;      // E
   float* sn = se + kC * kVS;      // N, then M + M^t
   float* sz = sn + kC * kS;       // Z, then M
-  float* sb = sz + kC * kS;
-  float* sbeta = sb + kC;
+  GateSum* sb = reinterpret_cast<GateSum*>(sz + kC * kS);
+  float* sbeta = reinterpret_cast<float*>(sb + kC);
   float* sr = sbeta + kC;         // r_i
   float* sc = sr + kC;            // c_j
   float* sdb = sc + kC;           // dU_j . E_j
@@ -344,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
       load_flat(s0, ks, w.S0 + ch * p.V * K + v0 * K, K, kVB, K, have);
       load_flat(s1, ks, w.dS1 + ch * p.V * K + v0 * K, K, kVB, K, have);
       __syncthreads();
-      const float end = sb[kC - 1];
+      const GateSum end = sb[kC - 1];
       product(fx, kVB, [&](int i, int v) { return sx[i * kVS + v]; }, [&](int v, int j) { return se[j * kVS + v]; });
       product(fn, kVB, [&](int i, int v) { return so[i * kVS + v]; }, [&](int v, int j) { return se[j * kVS + v]; });
       float acc[4][KJ];
@@ -352,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
       product(acc, kVB, [&](int i, int v) { return so[i * kVS + v]; }, [&](int v, int j) { return s0[v * ks + j]; });
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float f = p.scale * expf(sb[ty4 + i]);
+        const float f = p.scale * expf(sb[ty4 + i].hi);
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
           const float x = f * acc[i][j];
@@ -364,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
       product(acc, kVB, [&](int i, int v) { return sx[i * kVS + v]; }, [&](int v, int j) { return s0[v * ks + j]; });
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float f = -expf(sb[ty4 + i]);
+        const float f = -expf(sb[ty4 + i].hi);
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
           const float x = f * acc[i][j];
@@ -426,7 +421,7 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kThreads / 32; ++i) sum += sdot[i];
-      sum *= expf(sb[kC - 1]);
+      sum *= expf(sb[kC - 1].hi);
       for (int i = t; i < kC; ++i) {
         float x = sr[i];
         for (int j = 0; j < t; ++j) x += sz[i * kS + j];
@@ -463,10 +458,10 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const Params p, const B
   });
 }
 
-int smem_prep(int K) { return (2 * kC * (K + 1) + 2 * kC * kS + 2 * kC) * 4; }
-int smem_walk(int K) { return ((2 * kC + kVB) * (K + 1) + 2 * kC * kS + 2 * kC * kVS + 2 * kC) * 4; }
+int smem_prep(int K) { return (2 * kC * (K + 1) + 2 * kC * kS + 3 * kC) * 4; }
+int smem_walk(int K) { return ((2 * kC + kVB) * (K + 1) + 2 * kC * kS + 2 * kC * kVS + 3 * kC) * 4; }
 int smem_grads(int K) {
-  return ((2 * kC + 2 * kVB) * (K + 1) + 3 * kC * kVS + 2 * kC * kS + 5 * kC + kThreads / 32) * 4;
+  return ((2 * kC + 2 * kVB) * (K + 1) + 3 * kC * kVS + 2 * kC * kS + 6 * kC + kThreads / 32) * 4;
 }
 
 template <class F>

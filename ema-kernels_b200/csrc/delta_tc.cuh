@@ -21,15 +21,15 @@ namespace emab {
 namespace delta {
 
 constexpr int kTile = kC * 128;  // bytes of a 64-row, 128-byte-row region
-// gate record of a (chunk, head), 64 each: -exp(b_i), beta_i w_i, beta_i, b_i, key_j = exp(b_r - b_j), w_j = exp(b_end -
-// b_j); then exp(b_end) and, as bits 0, 8, 16, 24 of a word, the wide groups.  exp(b_i - b_j) = exp(b_i - b_r) key_j, r
+// gate record of a (chunk, head), 64 each: -exp(b_i), beta_i w_i, beta_i, b_i hi, key_j = exp(b_r - b_j), w_j = exp(b_end -
+// b_j), b_i lo; then exp(b_end) and, as bits 0, 8, 16, 24 of a word, the wide groups.  exp(b_i - b_j) = exp(b_i - b_r) key_j, r
 // the first token of j's 16-token group, except where a group is wide (its gates sum to more than kWideSpan, a reset
 // among them): there it is taken as it is.
 constexpr float kWideSpan = 60.f;
-constexpr int kGateFloats = 400;
+constexpr int kGateFloats = 464;
 constexpr uint32_t kStatusTmem = 0x200u;  // device status: a block that owns all of tensor memory did not get base 0
-constexpr int kGateE = 0, kGateW = 64, kGateBeta = 128, kGateB = 192, kGateKey = 256, kGateTail = 320, kGateEnd = 384,
-              kGateWide = 385;
+constexpr int kGateE = 0, kGateW = 64, kGateBeta = 128, kGateB = 192, kGateKey = 256, kGateTail = 320, kGateBLo = 384,
+              kGateEnd = 448, kGateWide = 449;
 
 struct TcBuffers {
   float* gates;      // kGateFloats per (slot, head)
