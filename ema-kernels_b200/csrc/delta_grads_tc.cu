@@ -4,7 +4,7 @@
 // With lanes as token rows (M = 128: 64 query rows over 64 key rows, [dO; dX] and [Q; K]) one chain gives both
 // 64 x 64 matrices of a head and one the products they are weighted with:
 //   [dO; dX] E^t = [f; F'],   [Q; K] K^t = [qk; kk]
-//   N = scale Gam f beta, M = -Gam F' beta (bf16, for dq and dk);  y = scale Gam f qk  over  -Gam F' kk
+//   N = scale Gam f beta, M = -Gam F' beta (bf16 pairs, for dq and dk);  y = scale Gam f qk  over  -Gam F' kk
 // with lanes as state columns (M = dstate) everything that ends in dq or dk:
 //   a1 = S0^t dO^t, a2 = S0^t dX^t, a3 = dS1^t E^t, a4 = K^t N^t, a5 = K^t (M + M^t) + Q^t N
 //   dq = scale exp(b) a1 + a4,   dk = -exp(b) a2 + beta w a3 + a5      (w_j = exp(b_end - b_j))
@@ -12,8 +12,8 @@
 //   dbeta_j = sum of y over its column + w_j k_j . a3_j
 //   dg_t = sum over rows of (prefix of beta y up to t) + sum_{i >= t} r_i + sum_{j < t} c_j + exp(b_end) <dS1, S0>
 // dg and dbeta are fp32 results, and sums that cancel: S0, dS1 and E enter as three bf16 pieces each, dX as two (dv and
-// the rest), with all products of them down to 2^-24.  N is a pair where it meets K for dq (whose two terms cancel where keys repeat); N and M for dk are
-// single bf16.
+// the rest), with all products of them down to 2^-24.  N and M are pairs: single bf16 would show beside the rounding of dk
+// itself (2.0e-3 off where that alone is 1.7e-3), and dq's two terms cancel where keys repeat.
 //
 // One block a SM, persistent over (chunk, group) and the group's heads, whose dq and dk add up in registers.  E's pieces
 // and dX's come as operand tiles, a head ahead.  S0 and dS1 come as fp32 images; warps 8-11 take them through registers in
@@ -80,11 +80,12 @@ struct Small {
 template <int K, int VP>
 struct Layout {
   static constexpr int ox = (K / 64) * kReg;             // after [Q; K]
-  static constexpr int ex = ox + (VP / 64) * kReg;       // E hi, mid, lo, dX lo, of this head and the next
-  static constexpr int kEx = 4 * VP * 128;
-  static constexpr int nm = ex + 2 * kEx;                // N, M
-  static constexpr int out = nm + 2 * kTile;             // N lo; 32 rows of dq or dk on their way out
-  static constexpr int small = out + kTile;              // (32 x dstate bf16 fit it)
+  static constexpr int ex = ox + (VP / 64) * kReg;       // E hi, mid, dX lo, of this head and the next
+  static constexpr int kEx = 3 * VP * 128;
+  static constexpr int el = ex + 2 * kEx;                // E lo, of one head as dO and dv are
+  static constexpr int nm = el + VP * 128;               // N hi, M hi, N lo, M lo: two tiles of 128 rows
+  static constexpr int out = nm + 2 * kTile;             // over N lo: 32 rows of dq or dk on their way out
+  static constexpr int small = nm + 4 * kTile;           // (32 x dstate bf16 fit a tile)
   static constexpr int bytes = small + static_cast<int>(sizeof(Small));
 };
 
@@ -186,12 +187,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(&bar.g_full[hc & 1], kGateFloats * 4);
           bulk_g2s(sm.gate[hc & 1], w.gates + ch * kGateFloats, kGateFloats * 4, &bar.g_full[hc & 1]);
           if (hc > 1 && !(ok = wait1(&bar.ex_empty[hc & 1], (hc / 2 - 1) & 1))) break;
-          mbar_arrive_expect_tx(&bar.ex_full[hc & 1], 4 * img);
+          mbar_arrive_expect_tx(&bar.ex_full[hc & 1], 3 * img);
           unsigned char* ex = smem + Lay::ex + (hc & 1) * Lay::kEx;
-          bulk_g2s(ex, w.E + ch * 3 * img, 3 * img, &bar.ex_full[hc & 1]);
-          bulk_g2s(ex + 3 * img, w.dX + ch * img, img, &bar.ex_full[hc & 1]);
+          bulk_g2s(ex, w.E + ch * 3 * img, 2 * img, &bar.ex_full[hc & 1]);
+          bulk_g2s(ex + 2 * img, w.dX + ch * img, img, &bar.ex_full[hc & 1]);
+          bulk_prefetch_l2(w.E + ch * 3 * img + 2 * img, img);
           if (hc > 0 && !(ok = wait1(&bar.ox_empty, last))) break;
-          mbar_arrive_expect_tx(&bar.ox_full, (VP / 64) * kReg);
+          mbar_arrive_expect_tx(&bar.ox_full, (VP / 64) * kReg + img);
+          bulk_g2s(smem + Lay::el, w.E + ch * 3 * img + 2 * img, img, &bar.ox_full);
           for (int i = 0; i < VP / 64; ++i) {
             tma_load_4d(smem + Lay::ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
             tma_load_4d(smem + Lay::ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idA = tc::idesc_bf16(128, 128, false, false);
       constexpr uint32_t idA64 = tc::idesc_bf16(128, 64, false, true);
       constexpr uint32_t idMM = tc::idesc_bf16(128, 64, true, true);
-      constexpr uint32_t idMK = tc::idesc_bf16(128, 64, true, false);
+      constexpr uint32_t idMK = tc::idesc_bf16(128, 128, true, false);
       auto kstep = [](int s) { return static_cast<uint32_t>(((s >> 2) * kReg + (s & 3) * 32) >> 4); };
       auto nstep = [](int s) { return static_cast<uint32_t>((s * 2048) >> 4); };
       auto jstep = [](int s) { return static_cast<uint32_t>((s * 32) >> 4); };
@@ -228,8 +231,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t dQK = desc_lo(sb, 16), dK = desc_lo(sb + kTile, 16);
       const uint32_t dQn = desc_lo(sb, qreg), dKn = desc_lo(sb + kTile, qreg);
       const uint32_t dOX = desc_lo(sb + Lay::ox, 16);
-      const uint32_t dN = desc_lo(sb + Lay::nm, 16), dM = desc_lo(sb + Lay::nm + kTile, 16);
-      const uint32_t dNl = desc_lo(sb + Lay::out, 16);
+      const uint32_t dN = desc_lo(sb + Lay::nm, 16), dM = desc_lo(sb + Lay::nm + kTile, 16);  // hi; M follows N
+      const uint32_t dNl = desc_lo(sb + Lay::nm + 2 * kTile, 16), dMl = desc_lo(sb + Lay::nm + 3 * kTile, 16);
+      const uint32_t dEl = desc_lo(sb + Lay::el, img);
       constexpr uint32_t im = img >> 4;  // from one piece of E to the next
       int n, tok, task = 0, hc = 0, rc = 0;
       Seq q;
@@ -241,8 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool cut = have < kC && p.cu != nullptr;  // rows of the next sequence in the tiles
         for (int h = 0; h < hpg; ++h, ++hc) {
           const uint32_t ph = hc & 1;
-          const uint32_t dE = desc_lo(sb + Lay::ex, img) + ph * (Lay::kEx >> 4);       // E hi, mid, lo, dX lo
-          const uint32_t dEX = desc_lo(sb + Lay::ex, 3 * img) + ph * (Lay::kEx >> 4);  // [E hi | dX lo]
+          const uint32_t dE = desc_lo(sb + Lay::ex, img) + ph * (Lay::kEx >> 4);       // E hi, mid, dX lo
+          const uint32_t dEX = desc_lo(sb + Lay::ex, 2 * img) + ph * (Lay::kEx >> 4);  // [E hi | dX lo]
           ok = wait(&bar.ox_full, ph) && wait(&bar.ex_full[ph], (hc >> 1) & 1);
           if (!ok) break;
           if (cut) {
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool more = s4 > 0 || i > 0;
                 mma_ss(tb + cF, ox + 2 * i, dE + vo + 128 * i, idF, more);
                 mma_ss(tb + cF, ox + 2 * i, dE + im + vo + 128 * i, idF, true);
-                mma_ss(tb + cF, ox + 2 * i, dE + 2 * im + vo + 128 * i, idF, true);
+                mma_ss(tb + cF, ox + 2 * i, dEl + vo + 128 * i, idF, true);
                 mma_ss(tb + cFX, dEX + vo + 128 * i, dE + vo + 128 * i, idMM, more);
                 mma_ss(tb + cFX, dEX + vo + 128 * i, dE + im + vo + 128 * i, idMM, true);
               }
@@ -306,14 +310,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma_ts_lo(tb + cA, aS, ox + 2 * i, idA, more);
                 mma_ts_lo(tb + cA, aS + pc, ox + 2 * i, idA, true);
                 mma_ts_lo(tb + cA, aS + 2 * pc, ox + 2 * i, idA, true);
-                mma_ts_lo(tb + cA + 64, aS, e + 3 * im, idA64, true);
-                mma_ts_lo(tb + cA + 64, aS + pc, e + 3 * im, idA64, true);
+                mma_ts_lo(tb + cA + 64, aS, e + 2 * im, idA64, true);
+                mma_ts_lo(tb + cA + 64, aS + pc, e + 2 * im, idA64, true);
                 mma_ts_lo(tb + cA3, aD, e, idA64, more);
                 mma_ts_lo(tb + cA3, aD + pc, e, idA64, true);
                 mma_ts_lo(tb + cA3, aD + 2 * pc, e, idA64, true);
                 mma_ts_lo(tb + cA3, aD, e + im, idA64, true);
                 mma_ts_lo(tb + cA3, aD + pc, e + im, idA64, true);
-                mma_ts_lo(tb + cA3, aD, e + 2 * im, idA64, true);
+                mma_ts_lo(tb + cA3, aD, dEl + vo + 128 * i, idA64, true);
                 tc::mma_commit(&bar.s_empty[i]);
               }
               __syncwarp();
@@ -331,11 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-              mma_ss(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);
+              mma_ss(tb + cF, dKn + nstep(s), dN + jstep(s), idMK, s > 0);  // K^t [N; M]^t: a4 and the first part of a5
               mma_ss(tb + cF, dKn + nstep(s), dNl + jstep(s), idMK, true);
-              mma_ss(tb + cFX, dKn + nstep(s), dM + jstep(s), idMK, s > 0);
               mma_ss(tb + cFX, dKn + nstep(s), dM + nstep(s), idMM, true);
+              mma_ss(tb + cFX, dKn + nstep(s), dMl + nstep(s), idMM, true);
               mma_ss(tb + cFX, dQn + nstep(s), dN + nstep(s), idMM, true);
+              mma_ss(tb + cFX, dQn + nstep(s), dNl + nstep(s), idMM, true);
             }
             tc::mma_commit(&bar.a45);  // and with them a1 to a3
             if (h == hpg - 1) tc::mma_commit(&bar.qk_empty);
@@ -560,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int m = 0; m < 4; ++m) split2(make_float2(R[8 * k + 2 * m], R[8 * k + 2 * m + 1]), o[m], l[m]);
               const uint32_t to = tc::chunk_off(i, cg / 8 + k);
               *reinterpret_cast<uint4*>(tile + to) = make_uint4(o[0], o[1], o[2], o[3]);
-              if (!second) *reinterpret_cast<uint4*>(smem + Lay::out + to) = make_uint4(l[0], l[1], l[2], l[3]);
+              *reinterpret_cast<uint4*>(tile + 2 * kTile + to) = make_uint4(l[0], l[1], l[2], l[3]);
             }
             // y, and the prefixes of beta y along the row that reach column t <= i
             float prod[16];
