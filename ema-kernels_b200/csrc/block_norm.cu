@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? 
       }
     const float2 sums = group_sum<TG>(sum, dot, buf, turn);
     // (past the end: 0, so that with eps = 0, whose rstd of an empty row is infinite, dw gets nothing from there either)
-    const float rstd = live ? rsqrtf(fmaf(sums.x, inv_m, p.eps)) : 0.f;
+    const float rstd = BWD && !live ? 0.f : rsqrtf(fmaf(sums.x, inv_m, p.eps));
     const float c1 = sums.y * rstd * inv_m;  // mean of d^ t^
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
