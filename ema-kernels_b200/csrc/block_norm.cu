@@ -56,8 +56,13 @@ struct Params {
   float* partial;  // (blocks, m) of this group's weight gradient, group-major
 };
 
-// (the approximate reciprocal is within 2 ulp, and 0 where exp(-v) overflows)
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// The approximate reciprocal is within 2 ulp, and 0 where exp(-v) overflows.  16-bit calls take the approximate exponential too
+// (2 + 1.2 |v| ulp of fp32, far below their rounding); in fp32 calls it would show (1.9e-6 of y at gates down to -30).
+template <class T>
+__device__ __forceinline__ float sigmoid(float v) {
+  const float e = std::is_same_v<T, float> ? expf(-v) : __expf(-v);
+  return __fdividef(1.f, 1.f + e);
+}
 
 __device__ __forceinline__ float load_weight(const void* w, int type, int i) {
   if (type == EMA_DTYPE_F32) return static_cast<const float*>(w)[i];
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? 
           sum = fmaf(t[j][k], t[j][k], sum);
           if (BWD) dot = fmaf(d * w[j][k], t[j][k], dot);
         } else {
-          sg[j][k] = sigmoid(z);
+          sg[j][k] = sigmoid<T>(z);
           const float s = z * sg[j][k];
           t[j][k] = FIRST ? a : a * s;
           sum = fmaf(t[j][k], t[j][k], sum);
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) norm_wide_kernel(const Params p) {
     for (int c = threadIdx.x; c < p.m; c += kThreads) {
       float t, z, d;
       at(c, t, z, d);
-      const float s = RES ? 1.f : z * sigmoid(z);
+      const float s = RES ? 1.f : z * sigmoid<T>(z);
       const float v = (RES || p.before) ? t : t * s;
       sum = fmaf(v, v, sum);
       if (BWD) dot = fmaf((p.before ? d * s : d) * load_weight(p.w, p.wtype, g0 + c), v, dot);
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) norm_wide_kernel(const Params p) {
           part[c] = fmaf(d, th, part[c]);
         }
       } else {
-        const float sg = sigmoid(z), s = z * sg;
+        const float sg = sigmoid<T>(z), s = z * sg;
         const float th = (p.before ? t : t * s) * rstd;
         if (!BWD) {
           static_cast<T*>(p.y)[row * p.sy + g0 + c] = from_f32<T>(th * w * (p.before ? s : 1.f));

@@ -1,4 +1,5 @@
-"""The block norms where a thread group works on several rows, or on none, against float64.  Tolerances as in test_block_norm_gpu."""
+"""The block norms where a thread group works on several rows, or on none, against float64; and gates far
+from zero in fp32.  Tolerances as in test_block_norm_gpu."""
 
 import pytest
 import torch
@@ -50,3 +51,18 @@ def test_several_rows_for_each_thread_group(rows, D, group, dt):
         e = do_.residual_norm(_f64(x), _f64(z), _f64(w), 1e-5, 0.7, _f64(h), _f64(dy), _f64(dy))
         for name, got in zip(("y", "dx", "dh_total", "dw"), (y, *torch.autograd.grad([y, h], [x, z, w], [dy, dy]))):
             _hold(name, got, e[name])
+
+
+@pytest.mark.parametrize("before", [True, False])
+def test_fp32_gates_far_from_zero(before):
+    """sigmoid(z) down to e^-30 keeps fp32's digits (the norm first: y carries it as a factor).  Each element is a
+    chain of some ten roundings and three functions of at most 2 ulp: 16 ulp."""
+    from kernels.block_norm import rms_norm_gated
+    x, z, w = _rand(11, (64, 128), (64, 128), (128,))
+    z = -30 * torch.sigmoid(z) - 1
+    x = torch.where(x.abs() < 0.1, torch.ones_like(x), x)
+    w = 1 + 0.2 * w.abs()
+    want = do_.gated_norm(_f64(x), _f64(z), _f64(w), 1e-30, 128, before)["y"]
+    got = _f64(rms_norm_gated(x, z, w, eps=1e-30, norm_before_gate=before))
+    rel = abs(got - want) / abs(want)
+    assert rel.max() <= 16 * 2.0 ** -24, rel.max()
