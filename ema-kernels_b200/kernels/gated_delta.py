@@ -271,7 +271,12 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
     return (o, final) if return_final_states else o
 
 
+_BLOCKS = "gated_delta_step: the (headdim, dstate) block of a state must be contiguous, 16-byte aligned and its own"
+
+
 def _delta_step(q, k, v, g, beta, states, state_indices, scale):
+    if states.data_ptr() & 15:  # (here: an address is nothing that a trace has)
+        raise ValueError(_BLOCKS)
     b, T, H, V = v.shape
     o = torch.empty(b, T, H, V, dtype=v.dtype, device=v.device)
     q, k, g, beta = _rows(q), _rows(k), _f32(g), _f32(beta)
@@ -318,10 +323,8 @@ def gated_delta_step(q, k, v, g, beta, states, scale=None, state_indices=None):
     if states.get_device() != v.get_device():
         raise ValueError("gated_delta_step: states must be on v's device")
     s0, s1, s2, s3 = states.stride()
-    if s3 != 1 or s2 != K or states.data_ptr() & 15 or (s0 | s1) & 3 or (
-            states.shape[0] > 1 and s0 < V * K) or (H > 1 and s1 < V * K):
-        raise ValueError("gated_delta_step: the (headdim, dstate) block of a state must be contiguous, 16-byte aligned "
-                         "and its own")
+    if s3 != 1 or s2 != K or s0 % 4 or s1 % 4 or (states.shape[0] > 1 and s0 < V * K) or (H > 1 and s1 < V * K):
+        raise ValueError(_BLOCKS)
     if state_indices is None:
         if states.shape[0] < b:
             raise ValueError(f"gated_delta_step: {b} rows on {states.shape[0]} slots")

@@ -1,0 +1,63 @@
+"""The delta rule and the block norms under torch.compile on the GPU: one graph (fullgraph=True, the aot_eager backend:
+the library's kernels are its operators), results equal to those of eager calls bit by bit."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import delta_oracle as do_
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _inputs(B, L, G=2, H=4, K=64, V=64, dt=torch.bfloat16, seed=0):
+    per = [do_.make_delta_inputs(L, G, H, K, V, seed + i) for i in range(B)]
+    t = [torch.from_numpy(np.stack([x[i] for x in per])).to(DEV) for i in range(6)]
+    return [t[0].to(dt), t[1].to(dt), t[2].to(dt), t[3], t[4]], t[5].to(dt)
+
+
+def _compiled(fn):
+    torch._dynamo.reset()
+    return torch.compile(fn, backend="aot_eager", fullgraph=True)
+
+
+@pytest.mark.parametrize("axis", [True, False])
+def test_compiled_step(axis):
+    from kernels.gated_delta import gated_delta_step
+    args, _ = _inputs(3, 1)
+    args = args if axis else [t[:, 0] for t in args]
+    states = torch.randn(5, 4, 64, 64, device=DEV)
+    at = torch.tensor([4, 9, 0], device=DEV)
+    ref, got = states.clone(), states.clone()
+    fn = lambda *a: gated_delta_step(*a[:-1], state_indices=a[-1])  # noqa: E731
+    want = fn(*args, ref, at)
+    o = _compiled(fn)(*args, got, at)
+    assert torch.equal(o, want) and torch.equal(got, ref) and not torch.equal(got, states)
+
+
+def test_step_refuses_states_off_16_bytes():
+    from kernels.gated_delta import gated_delta_step
+    args, _ = _inputs(2, 1)
+    off = torch.zeros(2 * 4 * 64 * 64 + 1, device=DEV)[1:].view(2, 4, 64, 64)
+    with pytest.raises(ValueError):
+        gated_delta_step(*args, off)
+    with pytest.raises(ValueError):
+        _compiled(lambda *a: gated_delta_step(*a))(*args, off)
+
+
+def test_compiled_norms():
+    from kernels.block_norm import residual_rms_norm, rms_norm_gated
+
+    def fn(x, z, h, w):
+        y, h = residual_rms_norm(x, h, w, scale=0.7)
+        return rms_norm_gated(y, z, w, group_size=64), h
+
+    leaves = [torch.randn(9, 128, device=DEV) for _ in range(3)] + [torch.ones(128, device=DEV)]
+    leaves[:2] = [t.bfloat16() for t in leaves[:2]]
+    runs = []
+    for f in (fn, _compiled(fn)):
+        xs = [t.clone().requires_grad_() for t in leaves]
+        y, h = f(*xs)
+        runs.append([y, h, *torch.autograd.grad([y, h], xs, [torch.ones_like(y), torch.ones_like(h)])])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
