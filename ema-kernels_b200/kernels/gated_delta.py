@@ -85,6 +85,13 @@ def _f32(t):
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
+def _saved_bytes(b, length, nseq, packed, H, V, K, code, flags):
+    """Bytes that a forward keeps for a backward: those of one (chunk, head), which the library knows, times their
+    number in plain arithmetic, so that a traced length stays a symbol."""
+    slots = length // 64 + nseq if packed else b * ((length + 63) // 64)
+    return slots * H * _lib.lib.delta_saved_bytes(1, 1, 0, 1, int(V), int(K), 1, code, flags)
+
+
 def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final, save):
     """One forward launch: (o, final states or None, what a backward needs or None)."""
     b, length, H, V = v.shape
@@ -96,8 +103,8 @@ def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_
     o = (torch.empty if cu_seqlens is None else torch.zeros)(b, length, H, V, dtype=v.dtype, device=dev)
     final = torch.empty(nseq, H, V, K, dtype=torch.float32, device=dev) if want_final else None
     s0 = None if initial_states is None else _f32(initial_states)
-    size = (b, length, nseq, H, V, K, G, code, flags)
-    n = _lib.lib.delta_saved_bytes(*size) if save else _lib.lib.delta_workspace_bytes(*size, 0)
+    n = (_saved_bytes(b, length, nseq, cu_seqlens is not None, H, V, K, code, flags) if save else
+         _lib.lib.delta_workspace_bytes(b, length, nseq, H, V, K, G, code, flags, 0))
     buf = torch.empty(n, dtype=torch.uint8, device=dev)
     at = buf.data_ptr()
     _fwd_launch(v.get_device(), b, length, H, V, K, G, nseq, code, scale, q.data_ptr(), *_strides3(q), k.data_ptr(),
@@ -149,7 +156,7 @@ def _(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags=0):
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
     nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    nbytes = _lib.lib.delta_saved_bytes(b, length, nseq, H, V, K, G, _lib.DTYPE_CODES[v.dtype], flags)
+    nbytes = _saved_bytes(b, length, nseq, cu_seqlens is not None, H, V, K, _lib.DTYPE_CODES[v.dtype], flags)
     return (v.new_empty((b, length, H, V)), v.new_empty((nseq, H, V, K), dtype=torch.float32),
             v.new_empty((nbytes,), dtype=torch.uint8))
 

@@ -61,3 +61,44 @@ def test_compiled_norms():
         y, h = f(*xs)
         runs.append([y, h, *torch.autograd.grad([y, h], xs, [torch.ones_like(y), torch.ones_like(h)])])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("packed", [False, True])
+def test_compiled_rule_trains_at_any_length(packed, dt):
+    """Forward, gradients and states; one compilation serves the lengths."""
+    from kernels.gated_delta import gated_delta_rule
+
+    def fn(q, k, v, g, beta, s0, cu):
+        return gated_delta_rule(q, k, v, g, beta, initial_states=s0, return_final_states=True,
+                                cu_seqlens=cu if packed else None)
+
+    compiled = _compiled(fn)
+    s0 = torch.randn(2, 4, 64, 64, device=DEV)
+    for L in (70, 131, 200):
+        args, do = _inputs(1 if packed else 2, L, dt=dt, seed=L)
+        for t in (*args, do):
+            torch._dynamo.mark_dynamic(t, 1)
+        cu = torch.tensor([0, 9, 70], device=DEV)
+        runs = []
+        for f in (fn, compiled):
+            xs = [t.detach().clone().requires_grad_() for t in (*args, s0)]
+            for t in xs[:5]:
+                torch._dynamo.mark_dynamic(t, 1)
+            o, fin = f(*xs, cu)
+            runs.append([o, fin, *torch.autograd.grad([o, fin], xs, [do, torch.ones_like(fin)])])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_opcheck_operators():
+    import kernels.block_norm  # noqa: F401
+    import kernels.gated_delta  # noqa: F401
+    args, _ = _inputs(2, 70)
+    xs = [t.requires_grad_() for t in args]
+    torch.library.opcheck(torch.ops.ema_b200.delta_fwd, (*xs, None, None, 1.0, 0),
+                          test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+    one, _ = _inputs(2, 1)
+    torch.library.opcheck(torch.ops.ema_b200.delta_step, (*one, torch.randn(3, 4, 64, 64, device=DEV), None, 1.0))
+    x, z, w = (torch.randn(*s, device=DEV).requires_grad_() for s in ((5, 64), (5, 64), (64,)))
+    torch.library.opcheck(torch.ops.ema_b200.gated_norm_fwd, (x, z, w, 1e-5, 32, True))
+    torch.library.opcheck(torch.ops.ema_b200.residual_norm_fwd, (x, z, w, 1e-5, 0.7))

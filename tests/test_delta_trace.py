@@ -61,3 +61,37 @@ def test_norms_trace(dynamic):
 
     ops, out = _trace(fn, make, dynamic)
     assert len(ops) == 2 and all(t.shape[1:] == (64,) for t in out)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_rule_traces_with_a_length_of_any_size(packed, dt):
+    """A length marked dynamic stays a symbol (marking it fails where the code makes a constant of it)."""
+    from kernels.gated_delta import gated_delta_rule
+
+    def make(mk):
+        a = _rule(mk, 1 if packed else 2, 70)
+        return [t.to(dt).requires_grad_() for t in a[:3]] + a[3:]
+
+    def fn(*a):
+        cu = torch.tensor([0, 9, 64], device="cuda") if packed else None
+        return gated_delta_rule(*a, return_final_states=True, cu_seqlens=cu)
+
+    ops, (o, fin) = _trace(fn, make, dynamic=1)
+    assert len(ops) == 1 and o.shape[2:] == (4, 64) and fin.shape == (2, 4, 64, 64)
+
+
+def test_bytes_kept_cover_what_the_library_needs():
+    """Python's number of bytes against the library's for the same chunk slots, and what it may exceed them by."""
+    from kernels import _lib
+    from kernels.gated_delta import _saved_bytes
+    for code in (0, 1, 2):
+        for H, V, K in ((1, 8, 64), (3, 72, 128), (4, 128, 128)):
+            for L in (1, 64, 65, 130, 4096):
+                got = _saved_bytes(2, L, 2, False, H, V, K, code, 0)
+                need = _lib.lib.delta_saved_bytes(2, L, 2, H, V, K, 1, code, 0)
+                assert need <= got <= 1.02 * need + 2048
+                for n in (1, 2, 9):
+                    got = _saved_bytes(1, L, n, True, H, V, K, code, 0)
+                    need = _lib.lib.delta_saved_bytes(1, L, n, H, V, K, 1, code, 0)
+                    assert need <= got <= 1.02 * need + 2048
