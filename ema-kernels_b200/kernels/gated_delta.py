@@ -161,6 +161,23 @@ def _(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags=0):
             v.new_empty((nbytes,), dtype=torch.uint8))
 
 
+@torch.library.custom_op("ema_b200::delta_infer", mutates_args=(), device_types="cuda")
+def _delta_infer_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                    initial_states: Optional[torch.Tensor], cu_seqlens: Optional[torch.Tensor], scale: float,
+                    flags: int, want_final: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """The forward that keeps nothing for a backward: (o, the final states, empty when not wanted)."""
+    o, final, _ = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final, False)
+    return o, final if want_final else _empty0(v)
+
+
+@_delta_infer_op.register_fake
+def _(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_final):
+    b, _, H, V = v.shape
+    nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    return (v.new_empty(v.shape), v.new_empty((nseq, H, V, k.shape[3]), dtype=torch.float32) if want_final
+            else _empty0(v))
+
+
 @torch.library.custom_op("ema_b200::delta_bwd", mutates_args=(), device_types="cuda")
 def _delta_bwd_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                   cu_seqlens: Optional[torch.Tensor], saved: torch.Tensor, do: torch.Tensor,
@@ -267,10 +284,15 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
                              f"{tuple(initial_states.shape)}")
     scale = K ** -0.5 if scale is None else float(scale)
     flags = _lib.DELTA_FP32_PRODUCTS if fp32_products else 0
+    train = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states))
     if torch.compiler.is_compiling():
-        o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags)
-    elif torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_states)):
+        if train:
+            o, final, _ = torch.ops.ema_b200.delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags)
+        else:
+            o, final = torch.ops.ema_b200.delta_infer(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags,
+                                                      return_final_states)
+    elif train:
         o, final = _Rule.apply(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, return_final_states)
     else:
         o, final, _ = _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, return_final_states,

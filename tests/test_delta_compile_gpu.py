@@ -90,13 +90,24 @@ def test_compiled_rule_trains_at_any_length(packed, dt):
         assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+@pytest.mark.parametrize("want", [False, True])
+def test_compiled_prefill(want):
+    from kernels.gated_delta import gated_delta_rule
+    args, _ = _inputs(2, 150)
+    fn = lambda *a: gated_delta_rule(*a, return_final_states=want)  # noqa: E731
+    a, b = fn(*args), _compiled(fn)(*args)
+    a, b = (a, b) if want else ([a], [b])
+    assert len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_opcheck_operators():
     import kernels.block_norm  # noqa: F401
     import kernels.gated_delta  # noqa: F401
     args, _ = _inputs(2, 70)
-    xs = [t.requires_grad_() for t in args]
+    xs = [t.clone().requires_grad_() for t in args]
     torch.library.opcheck(torch.ops.ema_b200.delta_fwd, (*xs, None, None, 1.0, 0),
                           test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+    torch.library.opcheck(torch.ops.ema_b200.delta_infer, (*args, None, None, 1.0, 0, True))
     one, _ = _inputs(2, 1)
     torch.library.opcheck(torch.ops.ema_b200.delta_step, (*one, torch.randn(3, 4, 64, 64, device=DEV), None, 1.0))
     x, z, w = (torch.randn(*s, device=DEV).requires_grad_() for s in ((5, 64), (5, 64), (64,)))

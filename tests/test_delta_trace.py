@@ -81,6 +81,26 @@ def test_rule_traces_with_a_length_of_any_size(packed, dt):
     assert len(ops) == 1 and o.shape[2:] == (4, 64) and fin.shape == (2, 4, 64, 64)
 
 
+@pytest.mark.parametrize("want", [False, True])
+def test_traced_inference_keeps_nothing_for_a_backward(want):
+    """147 KB a chunk and head otherwise, of a call that has no backward."""
+    from kernels.gated_delta import gated_delta_rule
+    fn = lambda *a: gated_delta_rule(*a, return_final_states=want)  # noqa: E731
+    ops, out = _trace(fn, _rule, dynamic=1)
+    assert len(ops) == 1 and "delta_infer" in ops[0]
+    if want:
+        assert out[1].shape == (2, 4, 64, 64)
+
+    def leaf(mk):
+        a = _rule(mk)
+        a[3].requires_grad_()
+        return a
+
+    assert "delta_fwd" in _trace(fn, leaf)[0][0]
+    with torch.no_grad():
+        assert "delta_infer" in _trace(fn, leaf)[0][0]
+
+
 def test_bytes_kept_cover_what_the_library_needs():
     """Python's number of bytes against the library's for the same chunk slots, and what it may exceed them by."""
     from kernels import _lib
