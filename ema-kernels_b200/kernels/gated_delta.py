@@ -277,7 +277,10 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
         if cu_seqlens.device != v.device:
             raise ValueError("gated_delta_rule: cu_seqlens must be on v's device")
         nseq = cu_seqlens.numel() - 1
-        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        if cu_seqlens.dtype == torch.int64:
+            # clamped before the narrowing, as the kernels clamp: past 32 bits an offset is still the call's end
+            cu_seqlens = cu_seqlens.clamp(0, length).to(torch.int32)
+        cu_seqlens = cu_seqlens.contiguous()
     if initial_states is not None:
         if initial_states.shape != (nseq, H, V, K) or initial_states.device != v.device:
             raise ValueError(f"gated_delta_rule: initial_states must be {(nseq, H, V, K)} on v's device, got "

@@ -1,5 +1,5 @@
 """The delta rule on layouts and calls beside the plain ones: views with heads before tokens, packed calls whose
-sequences leave tokens out, more chunks than blocks."""
+sequences leave tokens out, more chunks than blocks, indices of 64 bits."""
 
 import numpy as np
 import pytest
@@ -54,6 +54,14 @@ def test_tokens_outside_every_sequence(itype, dt):
     alone = _run([t[:, 5:70] for t in args], do[:, 5:70])
     for got, ref in zip(want, alone):
         assert torch.equal(got[:, 5:70], ref)
+
+
+def test_offsets_of_64_bits_are_clamped_not_cut():
+    """Past 32 bits an offset means the call's end, as it does below them."""
+    args, do = _inputs(100, 1, 2, 64, 64, torch.bfloat16, seed=3)
+    a = _run(args, do, cu_seqlens=torch.tensor([-2 ** 40, 30, 2 ** 32], device=DEV))
+    b = _run(args, do, cu_seqlens=torch.tensor([0, 30, 100], device=DEV))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 @pytest.mark.parametrize("G,H,K,V", [(16, 16, 128, 128), (16, 48, 64, 64)])
