@@ -374,4 +374,5 @@ def gated_delta_step(q, k, v, g, beta, states, scale=None, state_indices=None):
         o = torch.ops.ema_b200.delta_step(q, k, v, g, beta, states, state_indices, scale)
     else:
         o = _delta_step(q, k, v, g, beta, states, state_indices, scale)
+        torch.autograd.graph.increment_version(states)  # written in place: a backward that saved them has to know
     return o.squeeze(1) if squeeze else o
