@@ -306,6 +306,19 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
 _BLOCKS = "gated_delta_step: the (headdim, dstate) block of a state must be contiguous, 16-byte aligned and its own"
 
 
+def _overlap(n, s0, m, s1, size):
+    """Whether two of n x m blocks of ``size`` elements, s0 and s1 apart, share one (a step writes all of them at once)."""
+    if (n > 1 and s0 < size) or (m > 1 and s1 < size):
+        return True
+    if n <= 1 or m <= 1 or s0 >= (m - 1) * s1 + size or s1 >= (n - 1) * s0 + size:
+        return False
+    for j in range(1, m):  # neither axis steps over the whole of the other: j s1 against the multiples of s0 beside it
+        i, rest = divmod(j * s1, s0)
+        if (i < n and rest < size) or (i + 1 < n and s0 - rest < size):
+            return True
+    return False
+
+
 def _delta_step(q, k, v, g, beta, states, state_indices, scale):
     if states.data_ptr() & 15:  # (here: an address is nothing that a trace has)
         raise ValueError(_BLOCKS)
@@ -355,7 +368,7 @@ def gated_delta_step(q, k, v, g, beta, states, scale=None, state_indices=None):
     if states.get_device() != v.get_device():
         raise ValueError("gated_delta_step: states must be on v's device")
     s0, s1, s2, s3 = states.stride()
-    if s3 != 1 or s2 != K or s0 % 4 or s1 % 4 or (states.shape[0] > 1 and s0 < V * K) or (H > 1 and s1 < V * K):
+    if s3 != 1 or s2 != K or s0 % 4 or s1 % 4 or _overlap(states.shape[0], s0, H, s1, V * K):
         raise ValueError(_BLOCKS)
     if state_indices is None:
         if states.shape[0] < b:
