@@ -44,6 +44,9 @@ def _workspace(rows, dim, group, dev):
 
 def _gated_fwd(x, z, weight, eps, group_size, before):
     dim = x.shape[-1]
+    if dim // group_size > 65535 or dim > 1 << 30:
+        raise ValueError(f"rms_norm_gated: x of {dim} channels in groups of {group_size}: at most 65535 groups and 2^30 "
+                         "channels")
     x2, z2, w = _rows2d(x, dim), _rows2d(z, dim), weight.contiguous()
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     _gated_fwd_launch(x.get_device(), x2.shape[0], dim, group_size, _CODES[x.dtype], _CODES[w.dtype], before, eps,
@@ -174,6 +177,8 @@ class _Residual(torch.autograd.Function):
 
 def _residual_fwd(x, residual, weight, eps, scale):
     dim, dev = x.shape[-1], x.device
+    if dim > 1 << 30:
+        raise ValueError(f"residual_rms_norm: x of {dim} channels: at most 2^30")
     x2, w = _rows2d(x, dim), weight.contiguous()
     if residual is None:
         rdtype, rptr, rstride = x.dtype, 0, 0

@@ -97,6 +97,10 @@ def _delta_fwd(q, k, v, g, beta, initial_states, cu_seqlens, scale, flags, want_
     b, length, H, V = v.shape
     G, K = q.shape[2], q.shape[3]
     nseq = b if cu_seqlens is None else cu_seqlens.numel() - 1
+    # (the limits stand here: in the traced part they would bound a symbolic size)
+    if max(nseq, H) > 65535 or length > 1 << 30 or max(b * ((length + 63) // 64), length // 64 + nseq) > 1 << 24:
+        raise ValueError(f"gated_delta_rule: q, k and v of {nseq} sequences, {length} tokens and {H} heads: at most 65535 "
+                         "sequences and heads, 2^30 tokens and 2^24 chunks of 64")
     dev, code = v.device, _lib.DTYPE_CODES[v.dtype]
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), _f32(g), _f32(beta)
     # a packed call's tokens outside every sequence get zeros
@@ -320,9 +324,12 @@ def _overlap(n, s0, m, s1, size):
 
 
 def _delta_step(q, k, v, g, beta, states, state_indices, scale):
+    b, T, H, V = v.shape
+    if max(b, H) > 65535 or T > 1 << 20:
+        raise ValueError(f"gated_delta_step: v of {b} rows, {T} tokens and {H} heads: at most 65535 rows and heads and 2^20 "
+                         "tokens")
     if states.data_ptr() & 15:  # (here: an address is nothing that a trace has)
         raise ValueError(_BLOCKS)
-    b, T, H, V = v.shape
     o = torch.empty(b, T, H, V, dtype=v.dtype, device=v.device)
     q, k, g, beta = _rows(q), _rows(k), _f32(g), _f32(beta)
     if v.stride(3) != 1:
