@@ -302,6 +302,9 @@ lib.ema_version.restype = ctypes.c_char_p
 # struct.pack (the C layout, native alignment) instead of field by field through ctypes.
 
 
+_launched: set = set()  # indices of the devices that launchers have run on
+
+
 class Launcher:
     """One launcher of the library: ``Launcher(name, mirror, format)(device_index, *fields)``.
 
@@ -317,6 +320,7 @@ class Launcher:
         self._fn.argtypes = [ctypes.c_char_p, _ptr]
 
     def __call__(self, index, *fields):
+        _launched.add(index)
         args = self._pack(*fields)
         if torch._C._cuda_getDevice() == index:
             code = self._fn(args, torch._C._cuda_getCurrentRawStream(index))
@@ -379,9 +383,17 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 
 
 def device_status(clear: bool = False) -> int:
-    """OR of the status words of every workspace (synchronises).  Non-zero means a
-    device-side wait timed out (EMA_DEVSTATUS_* bits) and results are invalid."""
+    """OR of the status words of every workspace and of the delta-rule kernels on every
+    device that ran them (synchronises).  Non-zero means a device-side wait timed out
+    (EMA_DEVSTATUS_* bits) and results are invalid."""
     st = 0
+    for dev in sorted(_launched):
+        with torch.cuda.device(dev):
+            torch.cuda.synchronize(dev)
+            word = ctypes.c_uint32(0)
+            check(lib.delta_device_status(ctypes.byref(word), int(clear), stream_ptr(torch.device("cuda", dev))),
+                  "delta_device_status")
+            st |= word.value
     with _ws_lock:
         bufs = list(_ws.items())
     for (dev, sp), buf in bufs:

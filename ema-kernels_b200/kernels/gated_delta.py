@@ -325,7 +325,7 @@ def _overlap(n, s0, m, s1, size):
 
 def _delta_step(q, k, v, g, beta, states, state_indices, scale):
     b, T, H, V = v.shape
-    if max(b, H) > 65535 or T > 1 << 20:
+    if b > 65535 or H > 65535 or T > 1048576:
         raise ValueError(f"gated_delta_step: v of {b} rows, {T} tokens and {H} heads: at most 65535 rows and heads and 2^20 "
                          "tokens")
     if states.data_ptr() & 15:  # (here: an address is nothing that a trace has)
