@@ -49,6 +49,7 @@ struct Bars {
   uint64_t s, w, wx, dot, dv;    // epilogues done: dS, W, exp(b) dX, dO~ ready; dv staged
   uint64_t drain;
   uint32_t taddr, fail;
+  int issued;  // chunks whose loads were issued
 };
 
 template <int K>
@@ -133,8 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bulk_g2s(base + St::oP, w.P + ch * 2 * kTile, 2 * kTile, &bar.full[st]);
         bulk_g2s(base + St::oG, w.gates + ch * kGateFloats, kGateFloats * 4, &bar.full[st]);
       }
-      if (r < nc)  // failed: the copies in flight land before the block ends
-        for (int i = max(0, r - kStages); i < r; ++i) mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, status);
+      bar.issued = r;
     }
     if (warp == kMma) {  // ---- MMAs
       constexpr uint32_t id64 = tc::idesc_bf16(128, 64, false, false);   // Z
@@ -427,6 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (*fail != 0u && tid == 0)  // the copies in flight land before the block ends
+    for (int i = max(0, bar.issued - kStages); i < bar.issued; ++i)
+      mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, status);
   if (warp == kMma) {
     tc::tmem_relinquish();
     tc::tmem_dealloc(bar.taddr, 512);

@@ -60,6 +60,7 @@ struct Bars {
   uint64_t out_sync;       // meeting of the output warps (bounded, unlike a barrier instruction)
   uint64_t drain;          // MMAs still in flight after a failed wait
   uint32_t taddr, fail;
+  int issued;  // chunks whose loads were issued
 };
 
 __device__ __forceinline__ float2 pair(const float (&a)[2][16], int i) {
@@ -152,8 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_4d(base + St::oV, &mv, &bar.full[st], 0, h, q.t0 + c * kC, q.b);
         bulk_g2s(base + St::oG, w.gates + ch * kGateFloats, kGateFloats * 4, &bar.full[st]);
       }
-      if (c < nc)  // failed: the copies in flight land before the block ends
-        for (int i = max(0, c - kStages); i < c; ++i) mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, status);
+      bar.issued = c;
     }
     if (KEEP && warp == kStore && lane == 0) {  // ---- E's pieces
       for (int c = 0; c < nc && wait1(&bar.ek, c & 1); ++c) {
@@ -494,6 +494,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (*fail != 0u && tid == 0)  // the copies in flight land before the block ends
+    for (int i = max(0, bar.issued - kStages); i < bar.issued; ++i)
+      mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, status);
   if (warp == kMma) {
     tc::tmem_relinquish();
     tc::tmem_dealloc(bar.taddr, 512);

@@ -66,6 +66,7 @@ struct Bars {
   uint64_t epi_sync;           // meeting of the epilogue warps (bounded, unlike a barrier instruction)
   uint64_t drain;
   uint32_t taddr, fail;
+  int n_g, n_ex, n_ox, n_qk;  // loads issued
 };
 
 struct Small {
@@ -168,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     set_regs_down<kRegCtl>();
     if (warp == kLoad && lane == 0) {  // ---- loads
       int n, tok, task = 0, hc = 0;    // tasks and heads begun
+      int n_g = 0, n_ex = 0, n_ox = 0;
       Seq q;
       bool ok = true;
       for (int t = blockIdx.x; ok && t < tasks; t += gridDim.x) {
@@ -186,11 +188,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (hc > 1 && !(ok = wait1(&bar.g_empty[hc & 1], (hc / 2 - 1) & 1))) break;
           mbar_arrive_expect_tx(&bar.g_full[hc & 1], kGateFloats * 4);
           bulk_g2s(sm.gate[hc & 1], w.gates + ch * kGateFloats, kGateFloats * 4, &bar.g_full[hc & 1]);
+          ++n_g;
           if (hc > 1 && !(ok = wait1(&bar.ex_empty[hc & 1], (hc / 2 - 1) & 1))) break;
           mbar_arrive_expect_tx(&bar.ex_full[hc & 1], 3 * img);
           unsigned char* ex = smem + Lay::ex + (hc & 1) * Lay::kEx;
           bulk_g2s(ex, w.E + ch * 3 * img, 2 * img, &bar.ex_full[hc & 1]);
           bulk_g2s(ex + 2 * img, w.dX + ch * img, img, &bar.ex_full[hc & 1]);
+          ++n_ex;
           bulk_prefetch_l2(w.E + ch * 3 * img + 2 * img, img);
           if (hc > 0 && !(ok = wait1(&bar.ox_empty, last))) break;
           mbar_arrive_expect_tx(&bar.ox_full, (VP / 64) * kReg + img);
@@ -199,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d(smem + Lay::ox + i * kReg, &mo, &bar.ox_full, 64 * i, h, tt, q.b);
             tma_load_4d(smem + Lay::ox + i * kReg + kTile, &mdv, &bar.ox_full, 64 * i, h, tt, q.b);
           }
+          ++n_ox;
           if (h == gr * hpg) {  // Q and K, which the products with E do not need
             if (task > 0 && !(ok = wait1(&bar.qk_empty, (task - 1) & 1))) break;
             mbar_arrive_expect_tx(&bar.qk_full, (K / 64) * kReg);
@@ -210,10 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (!ok) {  // failed: what was begun lands before the block ends (each barrier's last phase, or an earlier one)
-        const long long t0 = clock64();
-        while (clock64() - t0 < kWaitLimitCycles / 100) __nanosleep(1000);
-      }
+      bar.n_g = n_g, bar.n_ex = n_ex, bar.n_ox = n_ox, bar.n_qk = task;
     }
     if (warp == kMma) {  // ---- MMAs
       constexpr uint32_t idKQ = tc::idesc_bf16(128, 64, false, false);
@@ -708,6 +710,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (*fail != 0u && tid == 0) {  // the copies in flight land before the block ends: each barrier's last phase
+    auto last = [&](uint64_t* b, int n) {
+      if (n > 0) mbar_wait_bounded(b, (n - 1) & 1, status);
+    };
+    for (int i = 0; i < 2; ++i) {
+      last(&bar.g_full[i], (bar.n_g + 1 - i) / 2);
+      last(&bar.ex_full[i], (bar.n_ex + 1 - i) / 2);
+    }
+    last(&bar.ox_full, bar.n_ox);
+    last(&bar.qk_full, bar.n_qk);
+  }
   if (warp == kMma) {
     tc::tmem_relinquish();
     tc::tmem_dealloc(bar.taddr, 512);

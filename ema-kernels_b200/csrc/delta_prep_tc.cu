@@ -251,6 +251,11 @@ __global__ void __launch_bounds__(kThreads, 4) prep_tc_kernel(const __grid_const
   }
   tc::fence_before_sync();
   const int failed = __syncthreads_or(!ok || s.fail != 0);
+  if (failed && warp == 0) {  // the copies and the product in flight end before the block does
+    mbar_wait_bounded(&s.full, 0, status);
+    mbar_wait_bounded(&s.mma, 0, status);
+    __syncwarp();
+  }
   if (warp == 0) {
     tc::tmem_relinquish();
     tc::tmem_dealloc(tb, 64);
