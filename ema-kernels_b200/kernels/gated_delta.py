@@ -267,9 +267,11 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_states=None, return_f
 
     Gradients: q, k, v, g, beta and initial_states; those of a group's q and k sum over its heads.  The states,
     all sums and both gate gradients are fp32.  bf16 calls run on the tensor cores with their 32-bit operands as
-    pairs or threes of bf16: 2^-16 of each, some 4e-6 of a state or gate gradient.  Where keys repeat and beta is near one,
-    the gate gradients are small differences of large terms and keep fewer digits; ``fp32_products`` then gives
-    those of fp32 arithmetic, at about seventeen times the time.  fp16 and fp32 calls are always fp32 products."""
+    pairs or threes of bf16: 2^-16 of each, 2e-6 to 4e-6 of a state or gate gradient (a plain fp32 form: 2e-7 to 4e-7).
+    Where keys repeat and beta is near one, the gate gradients are small differences of large terms and keep fewer
+    digits (130 equal keys at beta 0.98: 0.8 % of dg and 1.5e-4 of dbeta; at beta 0.9, 6e-4 and 5e-5);
+    ``fp32_products`` then gives those of fp32 arithmetic (0.06 % and 1.5e-6; 5e-5 and 1.2e-6), at about seventeen times
+    the time.  fp16 and fp32 calls are always fp32 products."""
     b, length, H, V, G, K = _check(q, k, v, g, beta, "gated_delta_rule")
     _check_headdim(V, 128, "gated_delta_rule")
     nseq = b
