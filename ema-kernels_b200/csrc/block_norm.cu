@@ -17,8 +17,11 @@
 // blocks by a second kernel in a fixed order (bitwise reproducible).  TG is the smallest of 8, 16, 32 and
 // 256 threads that hold a row: a row per warp or less needs shuffles only.  The layout goes by the width alone:
 // rows that do not start on 16 bytes are read element by element in the same places, so results do not
-// depend on strides.  Odd widths take VEC = 1 with 256 threads, rows beyond 8192 (odd: 2048) columns a form
-// that reads the row twice from L1 / L2.
+// depend on strides.  Widths that are no multiple of 8 take VEC = 1 with 256 threads, rows beyond 8192 (those: 2048)
+// columns a form that reads the row twice from L1 / L2.  Where a row does not fit its threads well the bytes in flight are
+// fewer (64 Mi bf16 elements, gated forward and backward: 4.9 and 4.6 TB/s at 128 columns, 4.5 and 4.0 at 2048, 2.8 and 2.6
+// at 1024, where half of the threads hold nothing, 3.1 and 2.1 at 8192, whose backward spills 360 bytes a thread with the gate
+// first and 48 without, 1.6 and 1.6 at 777, two bytes a load).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -159,7 +162,7 @@ __device__ __forceinline__ void write_partial(const Params& p, const float (&dw)
 // (of the next one where a row is longer) are issued before a row's arithmetic, raw, so that a 16-bit tensor costs four
 // registers a vector: the bytes in flight are what bounds it.  The gated pair at 8192 x 32 heads of 128: 202 and 396 us
 // without, 156 and 261 one row ahead, 146 and 251 two (5.5 and 5.3 TB/s; packed arithmetic, two channels an instruction,
-// made no difference); the residual pair at 32768 x 2048: 131 and 176 (6.1 TB/s).
+// made no difference); the residual pair at 32768 x 2048: 134 and 179 (6.0 TB/s).
 // FIRST: the norm comes before the gate.
 template <class T, class R, int TG, int VEC, int NV, bool RES, bool BWD, bool FIRST>
 __global__ void __launch_bounds__(kThreads, (NV * VEC <= 8 && sizeof(T) == 2) ? (BWD ? 2 : 3) : 1) norm_kernel(const Params p) {

@@ -7,7 +7,9 @@
 //
 // with w_j = exp(b_end - b_j) and dO~_i = scale exp(b_i) dO_i.  W, dX and dS are the chain; Y (from P and dO as they
 // lie in shared memory) and dO~ Q are ready before it needs them.  Operands that are not bf16 by nature are hi + lo
-// pairs (delta_tc.cuh), dO~, whose rounding stays in dS, three pieces.  dv = dX; for the gradient kernel dS at every chunk's
+// pairs (delta_tc.cuh), dO~, whose rounding stays in dS, three pieces.  exp(b) dX, whose rounding stays there too, is a pair:
+// it comes from the pairs W and T, and a third piece would take the error of d initial states from 2.2e-6 to 1.9e-6 for
+// four more steps in the chain.  dv = dX; for the gradient kernel dS at every chunk's
 // end is left as an fp32 image, and what dX has beyond dv as a bf16 tile.
 //
 // Bound: the chain's latency, as in the forward walk (three dependent MMA groups of about 900, 750 and 950 cycles with

@@ -11,8 +11,8 @@
 // for E and U P^t; w U, whose rounding stays in the state, is three pieces.  (o = scale exp(b) S Q^t
 // + U P^t ends in bf16, but where keys repeat its two terms cancel: hi parts alone left it 1e-2 off there.)
 //
-// Bound: the chain's latency, 6000 cycles a chunk at dstate 128 (16384 tokens of 32 heads of 128: 825 us, and 850 with the
-// state product in one piece; 40 sequences, 8111 tokens of 16 heads: 116): three
+// Bound: the chain's latency, 6000 cycles a chunk at dstate 128 (16384 tokens of 32 heads of 128: 856 us, 3 % more with the
+// state product in one piece; 40 sequences, 8111 tokens of 16 heads: 117): three
 // dependent MMA groups (about 1000, 640 and 950 cycles) with an epilogue after each (600, 750 and 980) and the hand-overs
 // between them; the products for o run in their shadow.  A training forward with a block on most SMs is near its bytes
 // instead: it writes S, E and o, 128 KB a chunk and head, and reads 96 (4 x 4096 x 32: 320 us, 5.8 TB/s; 250 without S).

@@ -20,9 +20,9 @@
 // steps of 16 value channels (one MMA step), sum <dS1, S0> on the way and write the pieces to tensor memory as the left
 // operand: a step whose left operand is there takes 14 + N / 2 cycles, from shared memory 48 + N / 2, and the pieces need
 // neither 48 KB nor a proxy fence.  (Through shared memory, with E as fp32 too, the kernel took 700 us at 4 x 4096 x 32
-// heads of 128 x 128; so, 565.)  Order of a head: F; the steps, and half-way the Q and K products of a new group, whose
+// heads of 128 x 128; so, 569.)  Order of a head: F; the steps, and half-way the Q and K products of a new group, whose
 // tiles arrive late; a4 and a5.  The next head's F runs under this one's epilogue of a1 to a3.  Bound: the staging warps, 8
-// steps of about 1500 cycles of loads, turns, splits and hand-overs a head, near 17000 in all; the tensor pipe has 9500, the
+// steps of about 1500 cycles of loads, turns, splits and hand-overs a head, near 17000 in all; the tensor pipe has 10000, the
 // epilogues 10000, and the bytes (S0 and dS1 are 2 x 64 KB) would allow 9000.  Roles: warps 0-7 epilogues (lane quarter
 // w % 4, column half w / 4), warps 8-11 staging, warp 12 the MMAs, warp 13 the loads, warp 14 dg and dbeta from the
 // epilogues' sums.  The long loops are kept rolled where they can be: at twice the code the block ran at a third of the

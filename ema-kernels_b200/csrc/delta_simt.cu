@@ -9,8 +9,8 @@
 // All operands are staged in shared memory as fp32 with rows padded to an odd stride (no bank conflicts by
 // row or by column); products are register tiles of 4 rows x every 16th column a thread.  Bound: the
 // shared-memory reads of those products, and on few chunks the walks' chain (2 x 333 tokens of 4 heads of 64 x 64 in fp32:
-// 127 and 114 us for 6 chunks, 21 us a chunk; preparation 47, gradients 122).  The tensor-core kernels serve bf16; this family serves fp32 and
-// fp16 inputs, whose split into bf16 pieces would cost more products than it saves or would not fit fp16's range.
+// 125 and 115 us for 6 chunks, 20 us a chunk; preparation 46, gradients 123).  The tensor-core kernels serve bf16; this family
+// serves fp32 and fp16 inputs (an fp16 number is a bf16 pair and an fp32 one three pieces, but no kernel stages them so).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
