@@ -32,9 +32,9 @@ from kernels.gated_delta import gated_delta_rule, gated_delta_step  # noqa: E402
 class DeltaBlock(nn.Module):
     """norm -> projections -> gated delta rule -> gated norm -> projection, on a bf16 branch and an fp32 stream."""
 
-    def __init__(self, width, nheads, headdim, ngroups, dstate, conv=2):
+    def __init__(self, width, nheads, headdim, ngroups, dstate):
         super().__init__()
-        self.nheads, self.headdim, self.ngroups, self.dstate, self.conv = nheads, headdim, ngroups, dstate, conv
+        self.nheads, self.headdim, self.ngroups, self.dstate = nheads, headdim, ngroups, dstate
         self.sizes = [ngroups * dstate, ngroups * dstate, nheads * headdim, nheads * headdim, 2 * nheads]
         bf = dict(bias=False, dtype=torch.bfloat16)
         self.norm_in = nn.Parameter(torch.ones(width))
